@@ -28,7 +28,8 @@ enum {
   PI05_ERR_CUDA = 3,          /* a CUDA runtime or driver call failed (see pi05_last_error) */
   PI05_ERR_NOT_BOUND = 4,     /* launch before bind */
   PI05_ERR_DEVICE_TIMEOUT = 5,/* a bounded device-side wait gave up; see pi05_status */
-  PI05_ERR_NO_DEVICE = 6      /* no usable sm_100 GPU */
+  PI05_ERR_NO_DEVICE = 6,     /* no usable sm_100 GPU */
+  PI05_ERR_PAGE_TABLE = 7     /* a page, a position or a length that a kernel read from device memory is out of range */
 };
 
 /* Number of input tensors and their fixed order (reference megakernel.py:21-25):
@@ -314,6 +315,73 @@ int pi05_prefill_partials(int sms, int max_tokens, int tokens, size_t* held, siz
 int pi05_prefill_status(pi05_prefill_t h, void* stream, int* code, int* where);
 const char* pi05_prefill_last_error(pi05_prefill_t h);
 int pi05_prefill_destroy(pi05_prefill_t h);
+
+/* ---- The prefix cache in pages, in BF16 or in 8 bits, and the attention of several sequences that share one prefix.
+ * (No counterpart in the reference: its cache is the dense pair of BF16 tensors that its prefill returns, reference/pi05.py:167-195, and every
+ * chunk attends over a prefix of its own, :254-265.)
+ *
+ * A cache is two pools, keys and values, [pages][layers][page_tokens][kv_heads][head_dim]; head_dim 64, 128 or 256, page_tokens a multiple
+ * of 16, pools and scales 16-byte aligned.  Formats: BF16; int8 and e4m3 with one FP32 scale per (token, head), [pages][layers][kv_heads]
+ * [page_tokens]: the value of an element is code x scale.  A sequence is a row of an int32 page table in device memory: its token t lies in page
+ * table[t / page_tokens] at t % page_tokens.  Tables, starts, counts and lengths are read by the kernels when they run, so they may change
+ * between launches and replays.  What they hold is checked there: the access is left out, and the status words of the cache (8 bytes of device
+ * memory, zero before the first call) keep the first such code and the sequence it came from.  Several calls on one cache may run at once where
+ * they touch different pages.  None of these functions waits (but for *_status) or takes device memory; all may be captured. */
+enum { PI05_CACHE_BF16 = 0, PI05_CACHE_INT8 = 1, PI05_CACHE_E4M3 = 2 };
+#define PI05_CACHE_BAD_PAGE 64         /* a page that is not in [0, pages) */
+#define PI05_CACHE_BAD_POSITION 65     /* a start or length that is negative or leads behind the sequence's last page */
+typedef struct pi05_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;            /* 8-bit formats */
+  unsigned int* status;                /* two words */
+  int format, pages, layers, page_tokens, kv_heads, head_dim;
+} pi05_cache;
+
+/* Rows of `batch` sequences x `layers` layers x `tokens` tokens: dense BF16 tensors of the caller's (k and v share their strides, in elements,
+ * multiples of 8; head_dim elements in a row; 16-byte aligned), which go with layers layer .. layer + layers - 1 of the cache and with the tokens
+ * starts[b] .. starts[b] + tokens - 1 of sequence b (starts = NULL: from 0).  counts (NULL: all): sequence b has only the first counts[b]
+ * of them. */
+typedef struct pi05_cache_rows {
+  void *k, *v;
+  long long batch_stride, layer_stride, token_stride, head_stride;
+  const int *table, *starts, *counts;  /* table [batch][table_stride >= table_pages] */
+  int batch, layers, tokens, layer, table_stride, table_pages;
+} pi05_cache_rows;
+
+/* Rows into their pages (k and v are read).  8 bits: scale = max|x| / 127 or / 448 over the head_dim elements of a token and head, in FP32; code =
+ * x / max|x| x 127 (448) to the nearest, the even one from the middle, of the true quotient.  A row of zeros has scale 0; one with an infinity or a NaN has
+ * scale NaN and reads back as NaN.  Rows behind counts[b] stay as they are.  Two rows of one call for the same place of the cache: either, or their
+ * codes and scales mixed. */
+int pi05_cache_write(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
+/* Rows out of their pages (k and v are written): code x scale in FP32, rounded to BF16.  Zeros behind counts[b]; NaN where a page or position is bad. */
+int pi05_cache_read(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
+/* Waits for `stream`, reads and clears the status words: PI05_ERR_PAGE_TABLE with code = PI05_CACHE_BAD_* and where = the sequence, or PI05_OK. */
+int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* code, int* where);
+
+/* Attention of batch x tokens queries over one prefix that all sequences share and over each sequence's own tokens:
+ *   out = sum_j p_j v_j,  p = softmax(scale q . k_j)  over the prefix tokens j < prefix_tokens with prefix_valid[j] != 0 (NULL: all) and the own
+ * tokens j < lengths[b] of sequence b; causal: own tokens j <= lengths[b] - tokens + t for query t, so that the queries are the last tokens
+ * of the sequence.  What masked places of the cache hold does not matter.  A query without any key gets zeros and lse -infinity.
+ * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8; query head h uses KV head
+ * h / (q_heads / kv_heads).  lse (NULL: not wanted): [batch][tokens][q_heads] FP32, the logarithm of the sum of exp(scale q . k_j).
+ * table = NULL: no own tokens.  Scores, softmax and sums are FP32; probabilities are rounded to BF16 (times the value's scale, 8 bits)
+ * before the product with the values.  A bad page makes the queries that see it NaN; lengths[b] out of range is cut to the nearest
+ * that is in it; both are reported in the status words of the cache. */
+typedef struct pi05_shared_call {
+  const void* q;
+  void* out;
+  float* lse;
+  long long q_batch_stride, q_token_stride, q_head_stride, out_batch_stride, out_token_stride, out_head_stride;
+  const int* prefix_table;             /* [ceil(prefix_tokens / page_tokens)] */
+  const unsigned char* prefix_valid;   /* [prefix_tokens] */
+  const int *table, *lengths;          /* [batch][table_stride >= table_pages], [batch] */
+  int batch, tokens, q_heads, layer, prefix_tokens, table_stride, table_pages, causal;
+  float scale;
+} pi05_shared_call;
+/* Bytes of device memory (256-byte aligned) that calls of up to max_batch x max_tokens queries need on a GPU of `sms` SMs.  Calls that share a
+ * workspace must not overlap. */
+int pi05_shared_workspace(int sms, const pi05_cache* cache, int q_heads, int max_batch, int max_tokens, size_t* bytes);
+int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared_call* call, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,9 @@ PREFILL_NUM_WEIGHTS = 9
 
 EVENT_ATTENTION_DONE, EVENT_FFN_NORM_READY = 7, 9
 WAIT_EVENT = 7
-OK, ERR_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_NOT_BOUND, ERR_DEVICE_TIMEOUT, ERR_NO_DEVICE = range(7)
+OK, ERR_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_NOT_BOUND, ERR_DEVICE_TIMEOUT, ERR_NO_DEVICE, ERR_PAGE_TABLE = range(8)
+CACHE_BF16, CACHE_INT8, CACHE_E4M3 = range(3)
+CACHE_BAD_PAGE, CACHE_BAD_POSITION = 64, 65
 
 _c = ctypes
 
@@ -32,6 +34,31 @@ class KvView(ctypes.Structure):
                 ("token_stride", _c.c_longlong), ("layer_stride", _c.c_longlong), ("page_stride", _c.c_longlong),
                 ("page_tokens", _c.c_int), ("num_pages", _c.c_int), ("pages_per_obs", _c.c_int),
                 ("page_table", _c.POINTER(_c.c_int))]
+
+
+class Cache(ctypes.Structure):
+    """``pi05_cache`` of the header: a cache in pages."""
+    _fields_ = [("k", _c.c_void_p), ("v", _c.c_void_p), ("k_scale", _c.c_void_p), ("v_scale", _c.c_void_p), ("status", _c.c_void_p),
+                ("format", _c.c_int), ("pages", _c.c_int), ("layers", _c.c_int), ("page_tokens", _c.c_int), ("kv_heads", _c.c_int),
+                ("head_dim", _c.c_int)]
+
+
+class CacheRows(ctypes.Structure):
+    """``pi05_cache_rows`` of the header: dense rows of keys and values and where they lie in a cache."""
+    _fields_ = [("k", _c.c_void_p), ("v", _c.c_void_p), ("batch_stride", _c.c_longlong), ("layer_stride", _c.c_longlong),
+                ("token_stride", _c.c_longlong), ("head_stride", _c.c_longlong), ("table", _c.c_void_p), ("starts", _c.c_void_p),
+                ("counts", _c.c_void_p), ("batch", _c.c_int), ("layers", _c.c_int), ("tokens", _c.c_int), ("layer", _c.c_int),
+                ("table_stride", _c.c_int), ("table_pages", _c.c_int)]
+
+
+class SharedCall(ctypes.Structure):
+    """``pi05_shared_call`` of the header: one attention over a shared prefix."""
+    _fields_ = [("q", _c.c_void_p), ("out", _c.c_void_p), ("lse", _c.c_void_p), ("q_batch_stride", _c.c_longlong),
+                ("q_token_stride", _c.c_longlong), ("q_head_stride", _c.c_longlong), ("out_batch_stride", _c.c_longlong),
+                ("out_token_stride", _c.c_longlong), ("out_head_stride", _c.c_longlong), ("prefix_table", _c.c_void_p),
+                ("prefix_valid", _c.c_void_p), ("table", _c.c_void_p), ("lengths", _c.c_void_p), ("batch", _c.c_int),
+                ("tokens", _c.c_int), ("q_heads", _c.c_int), ("layer", _c.c_int), ("prefix_tokens", _c.c_int), ("table_stride", _c.c_int),
+                ("table_pages", _c.c_int), ("causal", _c.c_int), ("scale", _c.c_float)]
 
 
 class Tuning(ctypes.Structure):
@@ -104,6 +131,11 @@ SIGNATURES = {
     "pi05_prefill_partials": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t), _c.POINTER(_c.c_size_t)]),
     "pi05_prefill_last_error": (_c.c_char_p, [_c.c_void_p]),
     "pi05_prefill_destroy": (_c.c_int, [_c.c_void_p]),
+    "pi05_cache_write": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.POINTER(CacheRows), _c.c_void_p]),
+    "pi05_cache_read": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.POINTER(CacheRows), _c.c_void_p]),
+    "pi05_cache_status": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
+    "pi05_shared_workspace": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
+    "pi05_shared_attention": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.POINTER(SharedCall), _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "pi05_tuning_defaults": (_c.c_int, [_c.POINTER(Tuning)]),
     "pi05_tune": (_c.c_int, [_c.c_void_p, _c.POINTER(Tuning)]),
     "pi05_chunk_static": (_c.c_int, [_c.c_int, _c.POINTER(_c.c_void_p), _c.c_int, _c.c_void_p, _c.c_int, _c.c_int,

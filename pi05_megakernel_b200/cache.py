@@ -1,0 +1,139 @@
+"""The prefix cache in pages, in BF16 or quantised to 8 bits as it is written.
+
+``KvCache`` holds pools of keys and values for any number of sequences: the prefix that ``Pi05Prefill`` produces, of one observation or of many,
+and the tokens that follow it.  ``write`` puts rows into the pages that a table names, ``read`` brings them back as the dense BF16 tensors that
+``Pi05Arm.bind`` takes; ``SharedPrefixAttention`` (shared.py) attends over the pages in place.  torch only supplies device memory and the
+current stream; the work is done by ``libpi05_b200.so``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+FORMATS = {"bf16": (_lib.CACHE_BF16, torch.bfloat16), "int8": (_lib.CACHE_INT8, torch.int8), "e4m3": (_lib.CACHE_E4M3, torch.float8_e4m3fn)}
+
+
+def check_table(name: str, t: torch.Tensor, device: torch.device, dim: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != dim or t.device != device or (t.numel() > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor of {dim} dimensions on {device}, contiguous along its last")
+
+
+def strides(t: torch.Tensor) -> list[int]:
+    """Strides of the dimensions but the last one; those of a single entry do not matter and are 0."""
+    return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+
+
+class KvCache:
+    """``pages`` pages of ``page_tokens`` tokens (a multiple of 16) for ``layers`` layers and ``kv_heads`` heads of ``head_dim`` (64, 128 or 256)
+    elements; ``format`` is ``"bf16"``, ``"int8"`` or ``"e4m3"``.
+
+    ``k`` and ``v`` are the pools ``[pages, layers, page_tokens, kv_heads, head_dim]``; of the 8-bit formats ``k_scale`` and ``v_scale``
+    ``[pages, layers, kv_heads, page_tokens]`` FP32 hold a scale per token and head, and an element stands for code x scale.  A BF16 cache of
+    one head of 256 is a pool that ``PagedPrefix`` takes as it is.
+    """
+
+    def __init__(self, pages: int, layers: int, page_tokens: int, kv_heads: int = 1, head_dim: int = 256, format: str = "int8",
+                 device: str = "cuda") -> None:
+        if format not in FORMATS:
+            raise ValueError(f"bad format {format!r}: expected one of {', '.join(FORMATS)}")
+        if min(pages, layers, kv_heads) < 1 or page_tokens < 16 or page_tokens % 16 or head_dim not in (64, 128, 256):
+            raise ValueError("a cache needs pages, layers and heads, pages of a multiple of 16 tokens, and heads of 64, 128 or 256 elements")
+        if not torch.cuda.is_available():
+            raise RuntimeError("no CUDA device: the cache has no CPU path")
+        shape = (pages, layers, page_tokens, kv_heads, head_dim)
+        pools = [torch.zeros(shape, dtype=FORMATS[format][1], device=device) for _ in range(2)]
+        scales = [None if format == "bf16" else torch.zeros((pages, layers, kv_heads, page_tokens), device=device) for _ in range(2)]
+        self._set(*pools, *scales)
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> "KvCache":
+        """A cache over pools that exist already (the shapes above, contiguous)."""
+        self = cls.__new__(cls)
+        self._set(k, v, k_scale, v_scale)
+        return self
+
+    def _set(self, k, v, k_scale, v_scale) -> None:
+        names = {dtype: name for name, (_, dtype) in FORMATS.items()}
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in names or k.device != v.device or k.device.type != "cuda":
+            raise ValueError("k and v must be CUDA tensors [pages, layers, page_tokens, kv_heads, head_dim] of one type: bfloat16, int8 or float8_e4m3fn")
+        self.pages, self.layers, self.page_tokens, self.kv_heads, self.head_dim = k.shape
+        self.format, self.device = names[k.dtype], k.device
+        want = (self.pages, self.layers, self.kv_heads, self.page_tokens)
+        for t in (k_scale, v_scale):
+            if (t is None) != (self.format == "bf16"):
+                raise ValueError("8-bit pools need scales, BF16 pools have none")
+            if t is not None and (tuple(t.shape) != want or t.dtype != torch.float32 or t.device != k.device):
+                raise ValueError(f"scales must be float32 {want} on {k.device}")
+        if not all(t is None or t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+            raise ValueError("pools and scales must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.lib = _lib.load()
+        self.words = torch.zeros(2, dtype=torch.int32, device=self.device)       # the status words
+        scale = (None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())
+        self.struct = _lib.Cache(k.data_ptr(), v.data_ptr(), *scale, self.words.data_ptr(), FORMATS[self.format][0], *k.shape)
+        self.ref = ctypes.byref(self.struct)
+        # what the library refuses is refused here, before a first call
+        nbytes = ctypes.c_size_t()
+        _lib.check(self.lib, None, self.lib.pi05_shared_workspace(1, self.ref, self.kv_heads, 1, 1, ctypes.byref(nbytes)))
+
+    def _rows(self, k, v, table, starts, counts, layer):
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != self.device or v.device != self.device:
+            raise ValueError(f"k and v must be bfloat16 [batch, layers, tokens, kv_heads, head_dim] on {self.device}")
+        batch, layers, tokens, heads, dim = k.shape
+        if heads != self.kv_heads or dim != self.head_dim or layer < 0 or layer + layers > self.layers:
+            raise ValueError(f"{tuple(k.shape)} from layer {layer} on does not fit a cache of {self.layers} layers x {self.kv_heads} heads of {self.head_dim}")
+        st = strides(k)
+        if st != strides(v) or k.stride(4) != 1 or v.stride(4) != 1 or any(s % 8 for s in st) or (k.data_ptr() | v.data_ptr()) % 16:
+            raise ValueError("k and v must share their strides (multiples of 8 elements, the last dimension contiguous) and be 16-byte aligned")
+        check_table("table", table, self.device, 2)
+        if table.shape[0] != batch:
+            raise ValueError("the page table needs a row per sequence")
+        for name, t in (("starts", starts), ("counts", counts)):
+            if t is not None:
+                check_table(name, t, self.device, 1)
+                if t.shape[0] != batch:
+                    raise ValueError(f"{name} needs an entry per sequence")
+        return _lib.CacheRows(k.data_ptr(), v.data_ptr(), *st, table.data_ptr(), None if starts is None else starts.data_ptr(),
+                              None if counts is None else counts.data_ptr(), batch, layers, tokens, layer, table.stride(0) if batch > 1 else table.shape[1],
+                              table.shape[1])
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor | None = None,
+              counts: torch.Tensor | None = None, layer: int = 0) -> None:
+        """Rows into their pages, asynchronous on the current stream.  ``k``, ``v`` BF16 ``[batch, layers, tokens, kv_heads, head_dim]`` of any
+        strides that they share go to layers ``layer`` .. of the cache and to the tokens ``starts[b]`` .. (None: 0 ..) of sequence ``b``, whose
+        pages ``table`` int32 ``[batch, pages]`` names; of a padded batch only the first ``counts[b]`` tokens are taken.  Tokens of one call must
+        lie in different places of the cache."""
+        rows = self._rows(k, v, table, starts, counts, layer)
+        _lib.check(self.lib, None, self.lib.pi05_cache_write(self.device.index, self.ref, ctypes.byref(rows),
+                                                             torch.cuda.current_stream(self.device).cuda_stream))
+
+    def read(self, table: torch.Tensor, tokens: int, starts: torch.Tensor | None = None, counts: torch.Tensor | None = None, layer: int = 0,
+             layers: int | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows out of their pages, asynchronous on the current stream: BF16 keys and values ``[batch, layers, tokens, kv_heads, head_dim]`` of
+        layers ``layer`` .. (all that there are), zeros behind ``counts[b]``; the rest as in ``write``."""
+        if out is None:
+            shape = (table.shape[0], self.layers - layer if layers is None else layers, tokens, self.kv_heads, self.head_dim)
+            out = (torch.empty(shape, dtype=torch.bfloat16, device=self.device), torch.empty(shape, dtype=torch.bfloat16, device=self.device))
+        elif out[0].shape[1:3] != (self.layers - layer if layers is None else layers, tokens):
+            raise ValueError("out does not have the layers and tokens that are read")
+        rows = self._rows(*out, table, starts, counts, layer)
+        _lib.check(self.lib, None, self.lib.pi05_cache_read(self.device.index, self.ref, ctypes.byref(rows),
+                                                            torch.cuda.current_stream(self.device).cuda_stream))
+        return out
+
+    def status(self) -> None:
+        """Synchronise the current stream; raises when a call met a page or a position out of range, or a device-side wait gave up, since the last
+        time it was asked."""
+        code, where = ctypes.c_int(), ctypes.c_int()
+        rc = self.lib.pi05_cache_status(self.device.index, self.ref, torch.cuda.current_stream(self.device).cuda_stream, ctypes.byref(code),
+                                        ctypes.byref(where))
+        if rc == _lib.ERR_PAGE_TABLE:
+            what = "page" if code.value == _lib.CACHE_BAD_PAGE else "start or length"
+            raise _lib.EngineError(rc, f"{what} out of range in " + (f"sequence {where.value}" if where.value >= 0 else "the shared prefix"))
+        if rc == _lib.ERR_DEVICE_TIMEOUT:
+            raise _lib.EngineError(rc, f"device wait kind {code.value} gave up in block {where.value >> 16}")
+        _lib.check(self.lib, None, rc)

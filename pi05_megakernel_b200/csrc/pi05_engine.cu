@@ -570,6 +570,7 @@ const char* pi05_error_string(int code) {
     case PI05_ERR_NOT_BOUND: return "engine has no bound inputs";
     case PI05_ERR_DEVICE_TIMEOUT: return "a device-side wait timed out";
     case PI05_ERR_NO_DEVICE: return "no usable sm_100 device";
+    case PI05_ERR_PAGE_TABLE: return "a page, position or length in device memory is out of range";
     default: return "unknown error";
   }
 }

@@ -1,0 +1,85 @@
+"""Attention of several sequences that share one prefix.
+
+``SharedPrefixAttention`` attends with the queries of a batch of sequences over the pages of one prefix, which are read once for the whole batch, and
+over the pages of every sequence's own tokens: a step of several candidates that continue from one observation, drafted tokens that are checked in
+one pass, or the tokens of several action chunks.  torch only supplies device memory and the current stream; the work is done by
+``libpi05_b200.so``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .cache import KvCache, check_table, strides
+
+
+class SharedPrefixAttention:
+    """For calls of up to ``max_batch`` sequences x ``max_tokens`` queries of ``q_heads`` heads over ``cache``.  One call at a time: the calls
+    share a workspace."""
+
+    def __init__(self, cache: KvCache, q_heads: int, max_batch: int, max_tokens: int = 1) -> None:
+        if q_heads < 1 or q_heads % cache.kv_heads or max_batch < 1 or max_tokens < 1:
+            raise ValueError(f"q_heads must be a multiple of the cache's {cache.kv_heads} heads, max_batch and max_tokens at least 1")
+        self.cache, self.q_heads, self.max_batch, self.max_tokens = cache, q_heads, max_batch, max_tokens
+        self.lib, self.device = cache.lib, cache.device
+        nbytes = ctypes.c_size_t()
+        sms = torch.cuda.get_device_properties(self.device).multi_processor_count
+        _lib.check(self.lib, None, self.lib.pi05_shared_workspace(sms, cache.ref, q_heads, max_batch, max_tokens, ctypes.byref(nbytes)))
+        self.ws = torch.zeros(nbytes.value, dtype=torch.uint8, device=self.device)
+
+    def run(self, q: torch.Tensor, prefix_table: torch.Tensor | None, prefix_tokens: int, table: torch.Tensor | None = None,
+            lengths: torch.Tensor | None = None, layer: int = 0, valid: torch.Tensor | None = None, causal: bool = True,
+            scale: float | None = None, out: torch.Tensor | None = None, with_lse: bool = False):
+        """Asynchronous on the current stream.  ``q`` BF16 ``[batch, tokens, q_heads, head_dim]`` of any strides; returns the outputs in the same
+        shape and, ``with_lse``, their log-sum-exp FP32 ``[batch, tokens, q_heads]``.
+
+        ``prefix_table`` int32 ``[pages]`` names the pages of the ``prefix_tokens`` shared tokens, ``valid`` bool ``[prefix_tokens]`` which
+        of them count (None: all).  ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` are the sequences' own tokens, the
+        queries' among them; ``causal``: query t sees own tokens up to its own place, ``lengths[b] - tokens + t``, else all of them.
+        ``scale`` defaults to head_dim ** -0.5.  A query that sees no key gets zeros (log-sum-exp: -infinity)."""
+        c = self.cache
+        if q.dim() != 4 or q.dtype != torch.bfloat16 or q.device != self.device or q.shape[2] != self.q_heads or q.shape[3] != c.head_dim:
+            raise ValueError(f"q must be bfloat16 [batch, tokens, {self.q_heads}, {c.head_dim}] on {self.device}")
+        batch, tokens = q.shape[:2]
+        if batch > self.max_batch or tokens > self.max_tokens:
+            raise ValueError(f"{batch} x {tokens} queries: made for up to {self.max_batch} x {self.max_tokens}")
+        if not 0 <= layer < c.layers or prefix_tokens < 0:
+            raise ValueError("no such layer in the cache, or a negative prefix_tokens")
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device:
+            raise ValueError("out must be like q")
+        qs, os_ = strides(q), strides(out)
+        if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_) or (q.data_ptr() | out.data_ptr()) % 16:
+            raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
+        if prefix_tokens:
+            if prefix_table is None:
+                raise ValueError("a prefix needs its page table")
+            check_table("prefix_table", prefix_table, self.device, 1)
+            if prefix_table.shape[0] * c.page_tokens < prefix_tokens:
+                raise ValueError("the prefix's page table is too short")
+            if valid is not None and (valid.dtype != torch.bool or tuple(valid.shape) != (prefix_tokens,) or not valid.is_contiguous() or valid.device != self.device):
+                raise ValueError(f"valid must be a contiguous bool tensor [{prefix_tokens}] on {self.device}")
+        if (table is None) != (lengths is None):
+            raise ValueError("own tokens need a table and lengths")
+        if table is not None:
+            check_table("table", table, self.device, 2)
+            check_table("lengths", lengths, self.device, 1)
+            if table.shape[0] != batch or lengths.shape[0] != batch:
+                raise ValueError("table and lengths need an entry per sequence")
+        lse = torch.empty((batch, tokens, self.q_heads), dtype=torch.float32, device=self.device) if with_lse else None
+        ptr = lambda t: None if t is None else t.data_ptr()
+        call = _lib.SharedCall(q.data_ptr(), out.data_ptr(), ptr(lse), *qs, *os_, ptr(prefix_table) if prefix_tokens else None,
+                               ptr(valid) if prefix_tokens else None, ptr(table), ptr(lengths), batch, tokens, self.q_heads, layer, prefix_tokens,
+                               0 if table is None else table.stride(0) if batch > 1 else table.shape[1], 0 if table is None else table.shape[1],
+                               bool(causal), c.head_dim ** -0.5 if scale is None else scale)
+        _lib.check(self.lib, None, self.lib.pi05_shared_attention(self.device.index, c.ref, ctypes.byref(call), self.ws.data_ptr(), self.ws.numel(),
+                                                                  torch.cuda.current_stream(self.device).cuda_stream))
+        return (out, lse) if with_lse else out
+
+    def status(self) -> None:
+        """``KvCache.status`` of the cache."""
+        self.cache.status()
