@@ -324,8 +324,8 @@ int pi05_prefill_destroy(pi05_prefill_t h);
  * of 16, pools and scales 16-byte aligned.  Formats: BF16; int8 and e4m3 with one FP32 scale per (token, head), [pages][layers][kv_heads]
  * [page_tokens]: the value of an element is code x scale.  A sequence is a row of an int32 page table in device memory: its token t lies in page
  * table[t / page_tokens] at t % page_tokens.  Tables, starts, counts and lengths are read by the kernels when they run, so they may change
- * between launches and replays.  What they hold is checked there: the access is left out, and the status words of the cache (8 bytes of device
- * memory, zero before the first call) keep the first such code and the sequence it came from.  Several calls on one cache may run at once where
+ * between launches and replays.  What they hold is checked there: the access is left out, and the status words of the cache (16 bytes of
+ * device memory, zero before the first call) keep the first such code and the sequence it came from (-1: the shared prefix).  Several calls on one cache may run at once where
  * they touch different pages.  None of these functions waits (but for *_status) or takes device memory; all may be captured. */
 enum { PI05_CACHE_BF16 = 0, PI05_CACHE_INT8 = 1, PI05_CACHE_E4M3 = 2 };
 #define PI05_CACHE_BAD_PAGE 64         /* a page that is not in [0, pages) */
@@ -333,7 +333,7 @@ enum { PI05_CACHE_BF16 = 0, PI05_CACHE_INT8 = 1, PI05_CACHE_E4M3 = 2 };
 typedef struct pi05_cache {
   void *k, *v;
   float *k_scale, *v_scale;            /* 8-bit formats */
-  unsigned int* status;                /* two words */
+  unsigned int* status;                /* four words: code and sequence; kind and block of a device-side wait that gave up */
   int format, pages, layers, page_tokens, kv_heads, head_dim;
 } pi05_cache;
 
@@ -355,7 +355,8 @@ typedef struct pi05_cache_rows {
 int pi05_cache_write(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
 /* Rows out of their pages (k and v are written): code x scale in FP32, rounded to BF16.  Zeros behind counts[b]; NaN where a page or position is bad. */
 int pi05_cache_read(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
-/* Waits for `stream`, reads and clears the status words: PI05_ERR_PAGE_TABLE with code = PI05_CACHE_BAD_* and where = the sequence, or PI05_OK. */
+/* Waits for `stream`, reads and clears the status words: PI05_ERR_PAGE_TABLE with code = PI05_CACHE_BAD_* and where = the
+ * sequence, PI05_ERR_DEVICE_TIMEOUT with code = the kind of wait and where = block << 16 (the call's outputs are NaN then), or PI05_OK. */
 int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* code, int* where);
 
 /* Attention of batch x tokens queries over one prefix that all sequences share and over each sequence's own tokens:
@@ -376,7 +377,7 @@ typedef struct pi05_shared_call {
   const unsigned char* prefix_valid;   /* [prefix_tokens] */
   const int *table, *lengths;          /* [batch][table_stride >= table_pages], [batch] */
   int batch, tokens, q_heads, layer, prefix_tokens, table_stride, table_pages, causal;
-  float scale;
+  float scale;                         /* positive */
 } pi05_shared_call;
 /* Bytes of device memory (256-byte aligned) that calls of up to max_batch x max_tokens queries need on a GPU of `sms` SMs.  Calls that share a
  * workspace must not overlap. */

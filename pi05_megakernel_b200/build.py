@@ -15,6 +15,7 @@ HEADERS = [os.path.join(HERE, "csrc", "ptx_sm100.cuh"), os.path.join(HERE, "csrc
            os.path.join(HERE, "csrc", "pi05_attention_o.cuh"),
            os.path.join(HERE, "csrc", "pi05_gemm.cuh"), os.path.join(HERE, "csrc", "pi05_steps.h"),
            os.path.join(HERE, "csrc", "pi05_ops.h"), os.path.join(HERE, "csrc", "pi05_cache.cuh"),
+           os.path.join(HERE, "csrc", "pi05_shared.cuh"),
            os.path.join(os.path.dirname(HERE), "include", "pi05_b200.h")]
 LIB = os.path.join(HERE, "libpi05_b200.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

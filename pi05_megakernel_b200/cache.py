@@ -72,7 +72,7 @@ class KvCache:
             raise ValueError("pools and scales must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.lib = _lib.load()
-        self.words = torch.zeros(2, dtype=torch.int32, device=self.device)       # the status words
+        self.words = torch.zeros(4, dtype=torch.int32, device=self.device)       # the status words
         scale = (None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())
         self.struct = _lib.Cache(k.data_ptr(), v.data_ptr(), *scale, self.words.data_ptr(), FORMATS[self.format][0], *k.shape)
         self.ref = ctypes.byref(self.struct)

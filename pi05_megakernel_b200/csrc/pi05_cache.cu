@@ -210,15 +210,16 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
   if (device < 0 || !cache::well_formed(cache) || !code || !where) return PI05_ERR_ARGUMENT;
   DeviceGuard guard(device);
   if (!guard.ok) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
-  unsigned int st[2] = {0, 0};
+  unsigned int st[4] = {0, 0, 0, 0};
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaMemcpyAsync(st, cache->status, sizeof st, cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaMemsetAsync(cache->status, 0, sizeof st, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return PI05_ERR_CUDA;
-  *code = (int)st[0];
-  *where = (int)st[1];
-  return !st[0] ? PI05_OK : st[0] < cache::BAD_PAGE ? PI05_ERR_DEVICE_TIMEOUT : PI05_ERR_PAGE_TABLE;
+  const unsigned int* first = st[2] ? st + 2 : st;       // a wait that gave up, else what was wrong with the tables
+  *code = (int)first[0];
+  *where = (int)first[1];
+  return st[2] ? PI05_ERR_DEVICE_TIMEOUT : st[0] ? PI05_ERR_PAGE_TABLE : PI05_OK;
 }
 
 }  // extern "C"

@@ -89,6 +89,27 @@ bool map_kv(CUtensorMap* m, const void* base, uint64_t tokens, uint64_t layers, 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool map_pages(CUtensorMap* m, const void* base, bool codes, uint64_t dim, uint64_t page_tokens, uint64_t heads, uint64_t layers, uint64_t pages,
+               uint64_t layer, uint32_t piece) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) return false;
+  const uint64_t size = codes ? 1 : 2, row = heads * dim * size, page = layers * page_tokens * row;
+  void* at = static_cast<uint8_t*>(const_cast<void*>(base)) + layer * page_tokens * row;
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  if (codes) {
+    cuuint64_t dims[4] = {dim, page_tokens, heads, pages};
+    cuuint64_t strides[3] = {row, dim, page};
+    cuuint32_t box[4] = {(cuuint32_t)dim, piece, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, at, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
+  cuuint64_t dims[5] = {64, page_tokens, dim / 64, heads, pages};
+  cuuint64_t strides[4] = {row, 128, dim * 2, page};
+  cuuint32_t box[5] = {64, piece, piece == 64 ? (cuuint32_t)(dim / 64) : 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, at, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The cheapest of the cuts that are built, by a model of the launch's time in SM cycles: rounds x 64-k blocks x the slower of the
 // tensor core (N / 2 cycles per K16 instruction) and shared memory (128 B per cycle: the rows of both operands that an
 // instruction reads, 64 or 128 of the activations, and the copies that bring them), not less than the weights' way from HBM

@@ -49,6 +49,11 @@ bool map_k(CUtensorMap* m, const void* base, uint64_t k, uint64_t rows, uint32_t
 bool map_kv(CUtensorMap* m, const void* base, uint64_t tokens, uint64_t layers, uint64_t pages, uint64_t token_stride,
             uint64_t layer_stride, uint64_t page_stride, uint32_t box_tokens, uint32_t box_blocks);
 
+// One layer of a pool of pages [pages][layers][page_tokens][heads][dim]: BF16 as {64 dims, page tokens, dim / 64, heads, pages}, box {64, piece, dim / 64 or, pieces
+// of less than 64 tokens, 1, 1, 1}, 128-byte swizzle; codes of a byte as {dim, page tokens, heads, pages}, box {dim, piece, 1, 1}, as they lie.
+bool map_pages(CUtensorMap* m, const void* base, bool codes, uint64_t dim, uint64_t page_tokens, uint64_t heads, uint64_t layers, uint64_t pages,
+               uint64_t layer, uint32_t piece);
+
 // How one projection of `tokens` x n features over k is cut.
 struct GemmPlan {
   int epi;            // gemm::EPI_*

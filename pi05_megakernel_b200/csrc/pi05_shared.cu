@@ -1,94 +1,26 @@
-// Attention of several sequences over one shared prefix and their own tokens, out of the pages of a cache.
+// Host side of the attention over a shared prefix: how a call is cut, tensor maps, launches.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
 
 #include "../../include/pi05_b200.h"
-#include "pi05_cache.cuh"
-#include "ptx_sm100.cuh"
+#include "pi05_ops.h"
+#include "pi05_shared.cuh"
 
 namespace {
 
-constexpr int WARPS = 8;
+using shared::Args;
 
-struct SharedArgs {
-  pi05_cache c;
-  pi05_shared_call s;
-};
-
-// One block per query row: its warps take every eighth key each, a lane DIM / 32 dims, and the parts are merged at the end.
-template <int FORMAT, int DIM>
-__global__ void __launch_bounds__(32 * WARPS) rows_kernel(const __grid_constant__ SharedArgs a) {
-  constexpr int E = DIM / 32;
-  const pi05_cache& c = a.c;
-  const pi05_shared_call& s = a.s;
-  __shared__ float s_m[WARPS], s_l[WARPS], s_o[WARPS][DIM];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % s.q_heads, bt = blockIdx.x / s.q_heads, t = bt % s.tokens, b = bt / s.tokens;
-  const int kh = h / (s.q_heads / c.kv_heads);
-  int length = s.table ? __ldg(s.lengths + b) : 0;
-  const long long most = (long long)s.table_pages * c.page_tokens;
-  if (length < 0 || length > most) {
-    if (threadIdx.x == 0) cache::report(c.status, cache::BAD_POSITION, b);
-    length = length < 0 ? 0 : (int)most;
-  }
-  int sees = s.causal ? length - s.tokens + t + 1 : length;
-  if (sees < 0) sees = 0;
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q) + b * s.q_batch_stride + t * s.q_token_stride + h * s.q_head_stride;
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) { qv[e] = __bfloat162float(q[lane * E + e]); o[e] = 0.f; }
-  auto value = [&](const void* pool, long long at, float scale, int e) {
-    if (FORMAT == PI05_CACHE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(pool)[at + e]);
-    const uint32_t w = static_cast<const uint8_t*>(pool)[at + e];
-    return cache::lo16(cache::pair<FORMAT == PI05_CACHE_BF16 ? PI05_CACHE_INT8 : FORMAT>(w)) * scale;
-  };
-  for (int j = warp; j < s.prefix_tokens + sees; j += WARPS) {
-    const bool own = j >= s.prefix_tokens;
-    if (!own && s.prefix_valid && !s.prefix_valid[j]) continue;
-    const int pos = own ? j - s.prefix_tokens : j, lp = pos / c.page_tokens, in = pos - lp * c.page_tokens;
-    const int page = own ? __ldg(s.table + (long long)b * s.table_stride + lp) : __ldg(s.prefix_table + lp);
-    if (page < 0 || page >= c.pages) {
-      if (lane == 0) cache::report(c.status, cache::BAD_PAGE, own ? b : -1);
-      m = l = NAN;
-      continue;
-    }
-    const long long pl = (long long)page * c.layers + s.layer;
-    const long long at = ((pl * c.page_tokens + in) * c.kv_heads + kh) * DIM + lane * E, sc = (pl * c.kv_heads + kh) * c.page_tokens + in;
-    const float ks = FORMAT == PI05_CACHE_BF16 ? 1.f : c.k_scale[sc], vs = FORMAT == PI05_CACHE_BF16 ? 1.f : c.v_scale[sc];
-    float x = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x += qv[e] * value(c.k, at, ks, e);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    x *= s.scale;
-    const float top = fmaxf(m, x), f = expf(m - top), p = expf(x - top);
-    m = top;
-    l = l * f + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * value(c.v, at, vs, e);
-  }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-#pragma unroll
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-  __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w]);
-  for (int w = 0; w < WARPS; ++w) L += s_m[w] == -INFINITY ? 0.f : s_l[w] * expf(s_m[w] - M);
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(s.out) + b * s.out_batch_stride + t * s.out_token_stride + h * s.out_head_stride;
-  for (int d = threadIdx.x; d < DIM; d += 32 * WARPS) {
-    float v = 0.f;
-    for (int w = 0; w < WARPS; ++w) v += s_m[w] == -INFINITY ? 0.f : s_o[w][d] * expf(s_m[w] - M);
-    out[d] = __float2bfloat16_rn(M == -INFINITY ? 0.f : v / L);
-  }
-  if (threadIdx.x == 0 && s.lse) s.lse[blockIdx.x] = M == -INFINITY ? -INFINITY : M + logf(L);
-}
-
-typedef void (*RowsKernel)(const SharedArgs);
-#define BY_DIM(F) {rows_kernel<F, 64>, rows_kernel<F, 128>, rows_kernel<F, 256>}
-const RowsKernel kRows[3][3] = {BY_DIM(PI05_CACHE_BF16), BY_DIM(PI05_CACHE_INT8), BY_DIM(PI05_CACHE_E4M3)};
+typedef void (*AttentionKernel)(const Args);
+typedef void (*CombineKernel)(const Args, int);
+#define BY_DIM(F) {shared::attention_kernel<F, 64>, shared::attention_kernel<F, 128>, shared::attention_kernel<F, 256>}
+const AttentionKernel kAttention[3][3] = {BY_DIM(PI05_CACHE_BF16), BY_DIM(PI05_CACHE_INT8), BY_DIM(PI05_CACHE_E4M3)};
 #undef BY_DIM
+const CombineKernel kCombine[3] = {shared::combine_kernel<64>, shared::combine_kernel<128>, shared::combine_kernel<256>};
 
 struct DeviceGuard {
   int prev = -1;
@@ -97,6 +29,24 @@ struct DeviceGuard {
   ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
+int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : 2; }
+long long up256(long long v) { return (v + 255) / 256 * 256; }
+
+// Tiles of query rows, and what unfinished items may leave behind: a slot per CTA and per item (a CTA's run ends at most one item early).
+struct Cut { long long a_tiles, b_tiles, b_rows, b_slot, a_bytes, b_bytes, plan_bytes; };
+Cut cut_rows(int sms, const pi05_cache& c, int q_heads, long long batch, long long tokens) {
+  const long long rows = tokens * (q_heads / c.kv_heads);
+  Cut k;
+  k.a_tiles = (batch * rows + shared::ROWS - 1) / shared::ROWS;
+  k.b_tiles = (rows + shared::ROWS - 1) / shared::ROWS;
+  k.b_rows = (rows + k.b_tiles - 1) / k.b_tiles;
+  k.b_slot = (k.b_rows + 3) / 4 * 4;
+  k.plan_bytes = up256((batch + 3) * 8);
+  k.a_bytes = up256((sms + k.a_tiles * c.kv_heads) * shared::ROWS * (c.head_dim + 2) * 4);
+  k.b_bytes = up256((sms + k.b_tiles * batch * c.kv_heads) * k.b_slot * (c.head_dim + 2) * 4);
+  return k;
+}
+
 }  // namespace
 
 extern "C" {
@@ -104,27 +54,76 @@ extern "C" {
 int pi05_shared_workspace(int sms, const pi05_cache* cache, int q_heads, int max_batch, int max_tokens, size_t* bytes) {
   if (sms < 1 || sms > 1024 || !cache::well_formed(cache) || q_heads < 1 || q_heads % cache->kv_heads || max_batch < 1 || max_tokens < 1 || !bytes)
     return PI05_ERR_ARGUMENT;
-  *bytes = 256;
+  if (max_batch > shared::MAX_BATCH || (long long)max_batch * max_tokens * q_heads > 0x7fffffffll) return PI05_ERR_UNSUPPORTED;
+  const Cut k = cut_rows(sms, *cache, q_heads, max_batch, max_tokens);
+  // fewer tokens may make the tiles of a sequence taller, up to all rows
+  const long long rows = std::min<long long>(shared::ROWS, ((long long)max_tokens * (q_heads / cache->kv_heads) + 3) / 4 * 4);
+  *bytes = (size_t)(k.plan_bytes + k.a_bytes + up256((sms + k.b_tiles * max_batch * cache->kv_heads) * rows * (cache->head_dim + 2) * 4));
   return PI05_OK;
 }
 
-int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared_call* call, void* workspace, size_t workspace_bytes, void* stream) {
-  if (device < 0 || !cache::well_formed(cache) || !call) return PI05_ERR_ARGUMENT;
+int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared_call* call, void* workspace, size_t workspace_bytes, void* stream_) {
+  if (device < 0 || device >= 64 || !cache::well_formed(cache) || !call) return PI05_ERR_ARGUMENT;
+  const pi05_cache& c = *cache;
   const pi05_shared_call& s = *call;
-  if (s.batch < 0 || s.tokens < 0 || s.q_heads < 1 || s.q_heads % cache->kv_heads || s.layer < 0 || s.layer >= cache->layers || s.prefix_tokens < 0)
+  if (s.batch < 0 || s.tokens < 0 || s.q_heads < 1 || s.q_heads % c.kv_heads || s.layer < 0 || s.layer >= c.layers || s.prefix_tokens < 0)
     return PI05_ERR_ARGUMENT;
   if (s.batch == 0 || s.tokens == 0) return PI05_OK;
-  if (!s.q || !s.out || (s.prefix_tokens && !s.prefix_table) || (s.table && (!s.lengths || s.table_pages < 0 || s.table_stride < 0))) return PI05_ERR_ARGUMENT;
-  if ((((uintptr_t)s.q | (uintptr_t)s.out) & 15) ||
-      ((s.q_batch_stride | s.q_token_stride | s.q_head_stride | s.out_batch_stride | s.out_token_stride | s.out_head_stride) & 7) ||
-      (((uintptr_t)s.lse | (uintptr_t)s.prefix_table | (uintptr_t)s.table | (uintptr_t)s.lengths) & 3))
+  if (!s.q || !s.out || !workspace || (s.prefix_tokens && !s.prefix_table) || (s.table && (!s.lengths || s.table_pages < 0 || s.table_stride < 0)))
     return PI05_ERR_ARGUMENT;
+  if ((((uintptr_t)s.q | (uintptr_t)s.out) & 15) || ((uintptr_t)workspace & 255) ||
+      ((s.q_batch_stride | s.q_token_stride | s.q_head_stride | s.out_batch_stride | s.out_token_stride | s.out_head_stride) & 7) ||
+      (((uintptr_t)s.lse | (uintptr_t)s.prefix_table | (uintptr_t)s.table | (uintptr_t)s.lengths) & 3) || !(s.scale > 0.f && s.scale < INFINITY))
+    return PI05_ERR_ARGUMENT;
+  if (s.batch > shared::MAX_BATCH || (long long)s.batch * s.tokens * s.q_heads > 0x7fffffffll) return PI05_ERR_UNSUPPORTED;
   DeviceGuard guard(device);
-  if (!guard.ok) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
-  const SharedArgs a = {*cache, s};
-  const RowsKernel kernel = kRows[cache->format][cache->head_dim == 64 ? 0 : cache->head_dim == 128 ? 1 : 2];
-  kernel<<<s.batch * s.tokens * s.q_heads, 32 * WARPS, 0, (cudaStream_t)stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? PI05_OK : PI05_ERR_CUDA;
+  int sms = 0;
+  if (!guard.ok || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
+  const Cut k = cut_rows(sms, c, s.q_heads, s.batch, s.tokens);
+  if ((long long)workspace_bytes < k.plan_bytes + k.a_bytes + k.b_bytes) return PI05_ERR_ARGUMENT;
+
+  Args a;
+  memset(&a, 0, sizeof a);
+  a.c = c; a.s = s;
+  a.group = s.q_heads / c.kv_heads;
+  a.piece = c.page_tokens % 64 == 0 ? 64 : c.page_tokens % 32 == 0 ? 32 : 16;
+  a.whole = a.piece == 64;
+  a.a_tiles = (int)k.a_tiles; a.b_tiles = (int)k.b_tiles; a.b_rows = (int)k.b_rows; a.b_slot = (int)k.b_slot;
+  a.p_tiles = (s.prefix_tokens + shared::TILE - 1) / shared::TILE;
+  // Prefix and own tokens as one list of keys where packing the batch's rows would not save a fifth of the tiles
+  a.joined = a.p_tiles == 0 || 4ll * s.batch * k.b_tiles <= 5 * k.a_tiles;
+  const long long own = s.table ? ((long long)s.table_pages * c.page_tokens + shared::TILE - 1) / shared::TILE : 0;
+  const long long most = c.kv_heads * ((a.joined ? 0 : k.a_tiles * (shared::OVERHEAD + a.p_tiles)) +
+                                       s.batch * k.b_tiles * (shared::OVERHEAD + own + (a.joined ? a.p_tiles : 0)));
+  a.grid = (int)std::min<long long>(sms, most);
+  a.c_log2 = s.scale * 1.4426950408889634f;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.plan = reinterpret_cast<long long*>(ws);
+  a.a_parts = reinterpret_cast<float*>(ws + k.plan_bytes);
+  a.b_parts = reinterpret_cast<float*>(ws + k.plan_bytes + k.a_bytes);
+  a.limit = 4000000000ll;
+  if (!pi05::map_pages(&a.k, c.k, c.format != PI05_CACHE_BF16, c.head_dim, c.page_tokens, c.kv_heads, c.layers, c.pages, s.layer, a.piece) ||
+      !pi05::map_pages(&a.v, c.v, c.format != PI05_CACHE_BF16, c.head_dim, c.page_tokens, c.kv_heads, c.layers, c.pages, s.layer, a.piece))
+    return PI05_ERR_CUDA;
+
+  const int d = dim_index(c.head_dim);
+  const AttentionKernel attention = kAttention[c.format][d];
+  const CombineKernel combine = kCombine[d];
+  const int smem = shared::smem_bytes(c.format, c.head_dim);
+  static std::atomic<uint64_t> done[3][3];
+  cudaError_t e = pi05::once_per_device(&done[c.format][d], device, [&] {
+    const cudaError_t first = pi05::chain_opt_in((const void*)attention, smem);
+    return first == cudaSuccess ? pi05::chain_opt_in((const void*)combine, 0) : first;
+  });
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (e == cudaSuccess) e = pi05::launch_kernel(attention, a.grid, shared::threads(c.format), smem, stream, 1, true, a);
+  // A row's parts are added by one warp, or by up to eight of a block where there are many: the CTAs' runs over the items they are shared by
+  const long long items = c.kv_heads * (a.joined ? s.batch * k.b_tiles : k.a_tiles), parts = a.grid / items + 1;
+  const int split = parts >= 16 ? 8 : parts >= 8 ? 4 : parts >= 4 ? 2 : 1;
+  const long long work = (long long)c.kv_heads * (((long long)s.batch * s.tokens * a.group + 7) / 8) * (c.head_dim / 16);
+  if (e == cudaSuccess) e = pi05::launch_kernel(combine, dim3((unsigned)((work * split + 7) / 8)), 256, 0, stream, 1, true, a, split);
+  if (e != cudaSuccess) { cudaGetLastError(); return PI05_ERR_CUDA; }
+  return PI05_OK;
 }
 
 }  // extern "C"

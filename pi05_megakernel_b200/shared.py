@@ -46,8 +46,9 @@ class SharedPrefixAttention:
         batch, tokens = q.shape[:2]
         if batch > self.max_batch or tokens > self.max_tokens:
             raise ValueError(f"{batch} x {tokens} queries: made for up to {self.max_batch} x {self.max_tokens}")
-        if not 0 <= layer < c.layers or prefix_tokens < 0:
-            raise ValueError("no such layer in the cache, or a negative prefix_tokens")
+        scale = c.head_dim ** -0.5 if scale is None else scale
+        if not 0 <= layer < c.layers or prefix_tokens < 0 or not 0 < scale < float("inf"):
+            raise ValueError("no such layer in the cache, a negative prefix_tokens, or a scale that is not positive and finite")
         if out is None:
             out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
         elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device:
@@ -75,7 +76,7 @@ class SharedPrefixAttention:
         call = _lib.SharedCall(q.data_ptr(), out.data_ptr(), ptr(lse), *qs, *os_, ptr(prefix_table) if prefix_tokens else None,
                                ptr(valid) if prefix_tokens else None, ptr(table), ptr(lengths), batch, tokens, self.q_heads, layer, prefix_tokens,
                                0 if table is None else table.stride(0) if batch > 1 else table.shape[1], 0 if table is None else table.shape[1],
-                               bool(causal), c.head_dim ** -0.5 if scale is None else scale)
+                               bool(causal), scale)
         _lib.check(self.lib, None, self.lib.pi05_shared_attention(self.device.index, c.ref, ctypes.byref(call), self.ws.data_ptr(), self.ws.numel(),
                                                                   torch.cuda.current_stream(self.device).cuda_stream))
         return (out, lse) if with_lse else out

@@ -63,7 +63,8 @@ def test_bad_rows_are_refused(lib, change):
 
 BAD_CALLS = [dict(q=None), dict(out=None), dict(q=0x60008), dict(out=0x70002), dict(q_heads=0), dict(q_heads=7), dict(layer=2), dict(layer=-1),
              dict(prefix_tokens=-1), dict(prefix_table=None), dict(lengths=None), dict(table_pages=-1), dict(batch=-1), dict(tokens=-1), dict(q_head_stride=4),
-             dict(out_token_stride=1), dict(lse=0x3), dict(table=0x90001), dict(prefix_table=0x80002)]
+             dict(out_token_stride=1), dict(lse=0x3), dict(table=0x90001), dict(prefix_table=0x80002), dict(scale=0.0),
+             dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))]
 
 
 @pytest.mark.parametrize("change", BAD_CALLS, ids=[str(c) for c in BAD_CALLS])
@@ -71,6 +72,21 @@ def test_bad_calls_are_refused(lib, change):
     assert lib.pi05_shared_attention(0, cache(), call(**change), 0x100000, 1 << 30, None) == _lib.ERR_ARGUMENT
     assert lib.pi05_shared_attention(0, cache(), None, 0x100000, 1 << 30, None) == _lib.ERR_ARGUMENT
     assert lib.pi05_shared_attention(-1, cache(), call(), 0x100000, 1 << 30, None) == _lib.ERR_ARGUMENT
+
+
+def test_workspace(lib):
+    """It grows with batch and tokens, holds any smaller call's, and a call refuses one that is too small, not aligned or missing."""
+    n, last = ctypes.c_size_t(), 0
+    for batch, tokens in ((1, 1), (2, 1), (2, 3), (16, 3), (16, 50), (1024, 50)):
+        assert lib.pi05_shared_workspace(148, cache(), 8, batch, tokens, n) == _lib.OK and n.value > last
+        last = n.value
+    assert lib.pi05_shared_workspace(148, cache(), 8, 1025, 1, n) == _lib.ERR_UNSUPPORTED
+    assert lib.pi05_shared_workspace(148, cache(), 8, 1024, 1 << 20, n) == _lib.ERR_UNSUPPORTED
+    assert lib.pi05_shared_workspace(148, cache(), 8, 0, 1, n) == _lib.ERR_ARGUMENT
+    assert lib.pi05_shared_workspace(148, cache(), 9, 1, 1, n) == _lib.ERR_ARGUMENT
+    assert lib.pi05_shared_attention(0, cache(), call(), None, 1 << 30, None) == _lib.ERR_ARGUMENT
+    assert lib.pi05_shared_attention(0, cache(), call(), 0x100010, 1 << 30, None) == _lib.ERR_ARGUMENT
+    assert lib.pi05_shared_attention(0, cache(), call(batch=1025), 0x100000, 1 << 30, None) == _lib.ERR_UNSUPPORTED
 
 
 def test_nothing_to_do_is_done(lib):
