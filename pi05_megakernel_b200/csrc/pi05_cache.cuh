@@ -17,29 +17,46 @@ __device__ __forceinline__ void report(unsigned int* status, int code, int where
   if (atomicCAS(status, 0u, (unsigned)code) == 0u) status[1] = (unsigned)where;
 }
 
-// Two codes in the low halves of the two bytes of each 16-bit half of `w` (0x00BB00AA) as a pair of BF16, exactly.
-//   int8: a code c = low - 128 * sign with low = c & 127.  0x4300 | low is 128 + low, 0x4300 | (c & 128) is 128 or 256, and the
-// difference of the two is exact.
+// Two codes of a byte as a pair of 16-bit numbers, exactly.  As BF16,
+//   int8: a code c is low - 128 sign with low = c & 127.  0x4300 | low is 128 + low, 0x4300 | (c & 128) is 128 or 256, and the difference of the
+// two is exact.  `w`: the codes in the low bytes of its halves.
 __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
   const uint32_t a = (w & 0x007f007fu) | 0x43004300u, b = (w & 0x00800080u) | 0x43004300u;
   uint32_t r;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-//   e4m3: exponent and mantissa moved to where BF16 has them read as the value times 2^-120, subnormals included, and the product with
-// 2^120 is exact.  (The two NaN codes read as 480: the kernels never write them.)
+//   e4m3: exponent and mantissa moved to where BF16 (FP16) has them read as the value times 2^-120 (2^-8), subnormals included, and the product
+// with 2^120 (2^8) is exact.  `w`: the codes in the high bytes of its halves, zeros in the low ones.  (The two NaN codes, which the kernels never write but
+// memory may hold at places that do not count, read as +-480.)
 __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
-  const uint32_t a = ((w & 0x007f007fu) << 4) | ((w & 0x00800080u) << 8);
+  const uint32_t a = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);
   uint32_t r;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x7b807b80u));
   return r;
 }
-template <int FORMAT>
-__device__ __forceinline__ uint32_t pair(uint32_t w) { return FORMAT == PI05_CACHE_INT8 ? int8_pair(w) : e4m3_pair(w); }
+__device__ __forceinline__ uint32_t e4m3_half_pair(uint32_t w) {
+  const uint32_t a = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x5c005c00u));
+  return r;
+}
 // Four codes of a word as two pairs of BF16.
 template <int FORMAT>
 __device__ __forceinline__ uint2 quad(uint32_t w) {
-  return make_uint2(pair<FORMAT>(__byte_perm(w, 0, 0x4140)), pair<FORMAT>(__byte_perm(w, 0, 0x4342)));
+  if (FORMAT == PI05_CACHE_INT8) return make_uint2(int8_pair(__byte_perm(w, 0, 0x4140)), int8_pair(__byte_perm(w, 0, 0x4342)));
+  return make_uint2(e4m3_pair(__byte_perm(w, 0, 0x1404)), e4m3_pair(__byte_perm(w, 0, 0x3424)));
+}
+// The same as FP16.  int8: 0x6400 | (c ^ 128) is 1024 + 128 + c.
+template <int FORMAT>
+__device__ __forceinline__ uint2 quad_half(uint32_t w) {
+  if (FORMAT != PI05_CACHE_INT8) return make_uint2(e4m3_half_pair(__byte_perm(w, 0, 0x1404)), e4m3_half_pair(__byte_perm(w, 0, 0x3424)));
+  uint2 r;
+  w ^= 0x80808080u;
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(a), "r"(0x64806480u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(b), "r"(0x64806480u));
+  return r;
 }
 
 __device__ __forceinline__ float lo16(uint32_t v) { return __uint_as_float(v << 16); }

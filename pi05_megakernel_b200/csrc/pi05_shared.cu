@@ -41,7 +41,7 @@ Cut cut_rows(int sms, const pi05_cache& c, int q_heads, long long batch, long lo
   k.b_tiles = (rows + shared::ROWS - 1) / shared::ROWS;
   k.b_rows = (rows + k.b_tiles - 1) / k.b_tiles;
   k.b_slot = (k.b_rows + 3) / 4 * 4;
-  k.plan_bytes = up256((batch + 3) * 8);
+  k.plan_bytes = up256((batch + 3) * 4);
   k.a_bytes = up256((sms + k.a_tiles * c.kv_heads) * shared::ROWS * (c.head_dim + 2) * 4);
   k.b_bytes = up256((sms + k.b_tiles * batch * c.kv_heads) * k.b_slot * (c.head_dim + 2) * 4);
   return k;
@@ -54,7 +54,7 @@ extern "C" {
 int pi05_shared_workspace(int sms, const pi05_cache* cache, int q_heads, int max_batch, int max_tokens, size_t* bytes) {
   if (sms < 1 || sms > 1024 || !cache::well_formed(cache) || q_heads < 1 || q_heads % cache->kv_heads || max_batch < 1 || max_tokens < 1 || !bytes)
     return PI05_ERR_ARGUMENT;
-  if (max_batch > shared::MAX_BATCH || (long long)max_batch * max_tokens * q_heads > 0x7fffffffll) return PI05_ERR_UNSUPPORTED;
+  if (max_batch > shared::MAX_BATCH || (long long)max_batch * max_tokens * q_heads > 1ll << 27) return PI05_ERR_UNSUPPORTED;
   const Cut k = cut_rows(sms, *cache, q_heads, max_batch, max_tokens);
   // fewer tokens may make the tiles of a sequence taller, up to all rows
   const long long rows = std::min<long long>(shared::ROWS, ((long long)max_tokens * (q_heads / cache->kv_heads) + 3) / 4 * 4);
@@ -75,7 +75,7 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
       ((s.q_batch_stride | s.q_token_stride | s.q_head_stride | s.out_batch_stride | s.out_token_stride | s.out_head_stride) & 7) ||
       (((uintptr_t)s.lse | (uintptr_t)s.prefix_table | (uintptr_t)s.table | (uintptr_t)s.lengths) & 3) || !(s.scale > 0.f && s.scale < INFINITY))
     return PI05_ERR_ARGUMENT;
-  if (s.batch > shared::MAX_BATCH || (long long)s.batch * s.tokens * s.q_heads > 0x7fffffffll) return PI05_ERR_UNSUPPORTED;
+  if (s.batch > shared::MAX_BATCH || (long long)s.batch * s.tokens * s.q_heads > 1ll << 27) return PI05_ERR_UNSUPPORTED;
   DeviceGuard guard(device);
   int sms = 0;
   if (!guard.ok || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
@@ -95,13 +95,14 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   const long long own = s.table ? ((long long)s.table_pages * c.page_tokens + shared::TILE - 1) / shared::TILE : 0;
   const long long most = c.kv_heads * ((a.joined ? 0 : k.a_tiles * (shared::OVERHEAD + a.p_tiles)) +
                                        s.batch * k.b_tiles * (shared::OVERHEAD + own + (a.joined ? a.p_tiles : 0)));
+  if (most > 0x3fffffffll) return PI05_ERR_UNSUPPORTED;
   a.grid = (int)std::min<long long>(sms, most);
   a.c_log2 = s.scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.plan = reinterpret_cast<long long*>(ws);
+  a.plan = reinterpret_cast<int*>(ws);
   a.a_parts = reinterpret_cast<float*>(ws + k.plan_bytes);
   a.b_parts = reinterpret_cast<float*>(ws + k.plan_bytes + k.a_bytes);
-  a.limit = 4000000000ll;
+  a.limit = 2000000000u;                        // about a second
   if (!pi05::map_pages(&a.k, c.k, c.format != PI05_CACHE_BF16, c.head_dim, c.page_tokens, c.kv_heads, c.layers, c.pages, s.layer, a.piece) ||
       !pi05::map_pages(&a.v, c.v, c.format != PI05_CACHE_BF16, c.head_dim, c.page_tokens, c.kv_heads, c.layers, c.pages, s.layer, a.piece))
     return PI05_ERR_CUDA;

@@ -11,10 +11,14 @@
 //   * The list (item, tile of 64 keys) of a launch is one sequence, cut into equal ranges, one per CTA, whatever the lengths are
 //     ("stream-K"): every CTA reads as many keys as any other.  A range that is not a whole item leaves unnormalised sums with their
 //     reference and weight, which combine_kernel adds in a fixed order: results do not depend on who is first.
-//   * Warp 0 copies (TMA), warp 1 issues the MMAs, warps 2 and 3 look pages and masks up ahead of both, warps 4-7 are the softmax, a
-//     thread per query row, and of an 8-bit cache warps 8-15 turn codes into BF16, exactly (pi05_cache.cuh).  A key's scale multiplies its score, a
-//     value's scale its probability, both in FP32.
-//   * The reference m of a row only moves when a score is more than 2^RESCALE above it; then the row's sums in tensor memory are rescaled.
+//   * Warp 0 copies (TMA), warp 1 issues the MMAs, warp 2 looks pages and masks up ahead of both.  Two groups of four warps are the softmax, a
+//     thread per query row, and take the tiles in turn: what a tile costs a group is mostly latency (tensor memory, barriers, the special
+//     functions of one warp per scheduler), which the other group's tile hides.  They share the reference m of a row, which goes from tile to
+//     tile in order; it only moves when a score is more than 2^RESCALE above it, and then the row's sums in tensor memory are rescaled.
+//   * Of an 8-bit cache two more groups turn codes into 16 bits, exactly: keys into BF16, as the queries are, values into FP16.  A key's scale
+//     multiplies its score and a value's scale its probability, both in FP32.  The product, rounded to FP16, keeps four bits more than
+//     BF16 would; so that it stays in FP16's range whatever the scales are, the reference of a row takes in the largest scale of
+//     the tile (warp 3 finds it): a shift that the division by the row's sum takes out again.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -27,20 +31,21 @@ namespace shared {
 
 constexpr int TILE = 64;                    // keys of a tile
 constexpr int ROWS = 128;                   // query rows of a tile
-constexpr int INFO = 8;                     // tiles that pages and masks are looked up ahead
-constexpr int OVERHEAD = 1;                 // what an item costs beside its tiles: loading Q, storing O
+constexpr int INFO = 16;                    // tiles that pages and masks are looked up ahead, in
+constexpr int BATCH = 8;                    // rounds of
+constexpr int OVERHEAD = 2;                 // what an item costs beside its tiles: loading Q, storing O
 constexpr int MAX_BATCH = 1024;
 constexpr float RESCALE = 8.0f;             // of exponents to the base 2: probabilities up to 256, their sums far from the ends of FP32
 
 __host__ __device__ constexpr int unit_bytes(int dim) { return TILE * dim * 2; }
 // Units (64 keys or values) of the BF16 ring and of the ring of codes in front of it.
-__host__ __device__ constexpr int units(int format, int dim) { return format == PI05_CACHE_BF16 ? (dim == 256 ? 6 : 12) : 4; }
-__host__ __device__ constexpr int raw_units(int format, int dim) { return format == PI05_CACHE_BF16 ? 0 : dim == 256 ? 5 : 10; }
+__host__ __device__ constexpr int units(int format, int dim) { return format == PI05_CACHE_BF16 ? (dim == 256 ? 6 : 12) : dim == 256 ? 4 : 8; }
+__host__ __device__ constexpr int raw_units(int format, int dim) { return format == PI05_CACHE_BF16 ? 0 : dim == 256 ? 4 : 8; }
 __host__ __device__ constexpr int scale_bytes(int format) { return format == PI05_CACHE_BF16 ? 0 : INFO * 2 * TILE * 4; }
 __host__ __device__ constexpr int smem_bytes(int format, int dim) {
-  return units(format, dim) * unit_bytes(dim) + raw_units(format, dim) * TILE * dim + scale_bytes(format) + (MAX_BATCH + 1) * 8 + 1024;
+  return units(format, dim) * unit_bytes(dim) + raw_units(format, dim) * TILE * dim + scale_bytes(format) + (2 * MAX_BATCH + 1) * 4 + 1024;
 }
-__host__ __device__ constexpr int threads(int format) { return format == PI05_CACHE_BF16 ? 256 : 512; }
+__host__ __device__ constexpr int threads(int format) { return format == PI05_CACHE_BF16 ? 384 : 640; }
 
 struct Args {
   CUtensorMap k, v;                         // BF16: {64 dims, page tokens, D / 64, heads, pages}; codes: {D, page tokens, heads, pages}
@@ -55,12 +60,12 @@ struct Args {
   int p_tiles;                              // tiles of the prefix
   int grid;
   float c_log2;                             // scale x log2 e
-  long long* plan;                          // what the combine kernel has to know: {units, CTAs, prefix sums of the sequences' units}
+  int* plan;                                // what the combine kernel has to know: {units, CTAs, prefix sums of the sequences' units}
   float *a_parts, *b_parts;                 // slots of unfinished items: [D / 4][rows][4], then (reference, weight) per row
-  long long limit;
+  uint32_t limit;                           // of a wait, in cycles
 };
 
-enum { WAIT_INFO = 1, WAIT_INFO_EMPTY, WAIT_RAW_EMPTY, WAIT_RAW_FULL, WAIT_KV_EMPTY, WAIT_KV_FULL, WAIT_Q, WAIT_S, WAIT_S_FREE, WAIT_P, WAIT_PV, WAIT_SCALES };
+enum { WAIT_INFO = 1, WAIT_INFO_EMPTY, WAIT_RAW_EMPTY, WAIT_RAW_FULL, WAIT_KV_EMPTY, WAIT_KV_FULL, WAIT_Q, WAIT_S, WAIT_S_FREE, WAIT_P, WAIT_PV, WAIT_SCALES, WAIT_O_FREE };
 
 // A run of tiles of one item.
 struct Segment {
@@ -70,62 +75,77 @@ struct Segment {
   int first, n, tiles;                      // tiles first .. first + n of `tiles`
 };
 
+// The launch's sequence of units: how it is cut, and where it comes from.
 struct Walk {
-  const long long* sums;                    // of the sequences' units, batch + 1
-  long long a_cost, a_units, b_units, units;
-  long long at, end;
-  int ctas;
+  const int* sums;                          // of the sequences' units, batch + 1
+  int a_cost, a_units, b_units, units, ctas;
+  int each, more;                           // units of a CTA; the first `more` have one more
 
-  __device__ __forceinline__ void set(const Args& p, const long long* s, int cta) {
+  __device__ __forceinline__ void cut(int u, int c) {
+    units = u; ctas = c;
+    each = c ? u / c : 0;
+    more = u - each * c;
+  }
+  __device__ __forceinline__ int begin(int cta) const { return cta < ctas ? cta * each + (cta < more ? cta : more) : units; }
+  __device__ __forceinline__ int cta_of(int unit) const {
+    const int big = more * (each + 1);
+    return unit < big ? unit / (each + 1) : more + (unit - big) / each;
+  }
+  __device__ __forceinline__ void set(const Args& p, const int* s) {
     sums = s;
     a_cost = OVERHEAD + p.p_tiles;
     a_units = p.joined ? 0 : a_cost * p.a_tiles * p.c.kv_heads;
     b_units = s[p.s.batch];
-    units = a_units + b_units * p.c.kv_heads;
-    ctas = units < p.grid ? (int)units : p.grid;
-    at = end = 0;
-    if (cta < ctas) { at = units * cta / ctas; end = units * (cta + 1) / ctas; }
-  }
-  __device__ __forceinline__ int cta_of(long long unit) const { return (int)(((unit + 1) * ctas - 1) / units); }
-  // The next run of this CTA that has tiles.
-  __device__ __forceinline__ bool next(const Args& p, Segment& g) {
-    while (at < end) {
-      long long off, cost;
-      if (at < a_units) {
-        g.batch = true;
-        g.item = (int)(at / a_cost);
-        off = at - g.item * a_cost;
-        cost = a_cost;
-        g.h = g.item / p.a_tiles;
-        g.r = g.item - g.h * p.a_tiles;
-        g.b = 0;
-        g.tiles = p.p_tiles;
-      } else {
-        g.batch = false;
-        const long long u = at - a_units;
-        g.h = (int)(u / b_units);
-        const long long w = u - g.h * b_units;
-        int lo = 0, hi = p.s.batch;         // the last sequence that begins at or before w (and has units)
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (sums[mid] <= w) lo = mid; else hi = mid;
-        }
-        g.b = lo;
-        cost = (sums[lo + 1] - sums[lo]) / p.b_tiles;
-        g.r = (int)((w - sums[lo]) / cost);
-        off = w - sums[lo] - g.r * cost;
-        g.item = (g.h * p.s.batch + g.b) * p.b_tiles + g.r;
-        g.tiles = (int)cost - OVERHEAD;
-      }
-      const long long last = off + (end - at) < cost ? off + (end - at) : cost;      // units of the item before `end`
-      g.first = off > OVERHEAD ? (int)off - OVERHEAD : 0;
-      g.n = (int)last - OVERHEAD - g.first;
-      at += last - off;
-      if (g.n > 0) return true;
-    }
-    return false;
+    const int u = a_units + b_units * p.c.kv_heads;
+    cut(u, u < p.grid ? u : p.grid);
   }
 };
+
+// The next run of this CTA that has tiles, from unit `at` on, to *out, by a whole warp; returns the unit behind it, or -1: there is none.  (One function
+// for all warps: what they execute does not fit the instruction cache many times.)
+static __device__ __noinline__ int next_segment(const Args& p, const Walk& w, int at, Segment* out) {
+  const int end = w.begin(blockIdx.x + 1);
+  Segment g;
+  g.n = 0;
+  while (at < end && g.n <= 0) {
+    int off, cost;
+    if (at < w.a_units) {
+      g.batch = true;
+      g.item = at / w.a_cost;
+      off = at - g.item * w.a_cost;
+      cost = w.a_cost;
+      g.h = g.item / p.a_tiles;
+      g.r = g.item - g.h * p.a_tiles;
+      g.b = 0;
+      g.tiles = p.p_tiles;
+    } else {
+      g.batch = false;
+      const int u = at - w.a_units;
+      g.h = u / w.b_units;
+      const int x = u - g.h * w.b_units;
+      int lo = 0, hi = p.s.batch;           // the last sequence that begins at or before x (and has units)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (w.sums[mid] <= x) lo = mid; else hi = mid;
+      }
+      g.b = lo;
+      off = x - w.sums[lo];
+      cost = w.sums[lo + 1] - w.sums[lo];
+      g.r = 0;
+      if (p.b_tiles > 1) { cost /= p.b_tiles; g.r = off / cost; off -= g.r * cost; }
+      g.item = (g.h * p.s.batch + g.b) * p.b_tiles + g.r;
+      g.tiles = cost - OVERHEAD;
+    }
+    const int last = off + (end - at) < cost ? off + (end - at) : cost;      // units of the item before `end`
+    g.first = off > OVERHEAD ? off - OVERHEAD : 0;
+    g.n = last - OVERHEAD - g.first;
+    at += last - off;
+  }
+  __syncwarp();
+  if (g.n > 0 && (threadIdx.x & 31) == 0) *out = g;
+  __syncwarp();
+  return g.n > 0 ? at : -1;
+}
 
 // Which sequence, token and query head row `row` of a tile is; false: none.
 __device__ __forceinline__ bool row_of(const Args& p, const Segment& g, int row, int& b, int& t, int& head) {
@@ -151,11 +171,16 @@ __device__ __forceinline__ int own_length(const Args& p, int b) {
   return n < 0 ? 0 : n > most ? (int)most : n;
 }
 
-// A operand from tensor memory, B from shared memory: one MMA of K = 16.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t accumulate, uint32_t on) {
-  asm volatile("{\n.reg .pred p, q;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\nmov.b64 db, {%2, %6};\n"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}"
-               ::"r"(d), "r"(a), "r"(blo), "r"(idesc), "r"(accumulate), "r"(on), "n"(ptx::UMMA_DESC_HI) : "memory");
+// Four MMAs of K = 16, the A operand from tensor memory, B from shared memory: 8 columns and STEP descriptor units further each.
+template <int STEP>
+__device__ __forceinline__ void umma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t accumulate, uint32_t on) {
+#define PI05_UMMA1(P0) "mov.b64 db, {bl, %6};\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [aa], db, %3, " P0 ";\n"
+#define PI05_UMMA_STEP "add.u32 bl, bl, %7;\n add.u32 aa, aa, 8;\n"
+  asm volatile("{\n.reg .pred p, q, t;\n.reg .b32 aa, bl;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\nsetp.eq.b32 t, 0, 0;\n"
+               "mov.b32 aa, %1;\nmov.b32 bl, %2;\n" PI05_UMMA1("p") PI05_UMMA_STEP PI05_UMMA1("t") PI05_UMMA_STEP PI05_UMMA1("t") PI05_UMMA_STEP PI05_UMMA1("t") "}"
+               ::"r"(d), "r"(a), "r"(blo), "r"(idesc), "r"(accumulate), "r"(on), "n"(ptx::UMMA_DESC_HI), "n"(STEP) : "memory");
+#undef PI05_UMMA1
+#undef PI05_UMMA_STEP
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -173,40 +198,113 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-// What warps 2 and 3 say about a tile.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long ra, rb, rd;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long ra, rb, rd;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
+  return d;
+}
+
+// Bounded wait of a converged warp on a barrier; one that gives up is reported and returns when what the CTA may still have in flight has finished.
+static __device__ __noinline__ bool wait_slow(const Args& p, uint32_t bar, uint32_t parity, int kind) {
+  const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+  do {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+  } while (!__any_sync(0xffffffffu, (uint32_t)clock() - t0 > p.limit));
+  if ((threadIdx.x & 31) == 0 && atomicCAS(p.c.status + 2, 0u, (unsigned)kind) == 0u) p.c.status[3] = blockIdx.x << 16;
+  const uint32_t t1 = (uint32_t)clock();
+  while ((uint32_t)clock() - t1 < 200000u) __nanosleep(1000);
+  __syncwarp();
+  return false;
+}
+__device__ __forceinline__ bool wait(const Args& p, uint32_t bar, uint32_t parity, int kind) {
+  return __all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity)) || wait_slow(p, bar, parity, kind);
+}
+
+// The queries of a softmax warp's 32 rows, as they lie, into tensor memory.
+template <int DIM>
+__device__ __noinline__ void load_queries(const Args& p, const Segment& s, int row, uint32_t columns) {
+  int b = 0, t = 0, head = 0;
+  const bool mine = row_of(p, s, row, b, t, head);
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.s.q) + b * p.s.q_batch_stride + t * p.s.q_token_stride + head * p.s.q_head_stride);
+#pragma unroll 1
+  for (int c = 0; c < DIM / 64; ++c) {
+    uint32_t w[32];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint4 x = mine ? __ldcg(q + c * 8 + j) : make_uint4(0u, 0u, 0u, 0u);
+      w[4 * j] = x.x; w[4 * j + 1] = x.y; w[4 * j + 2] = x.z; w[4 * j + 3] = x.w;
+    }
+    tmem_st_32x32(columns + 32 * c, w);
+  }
+  ptx::tmem_wait_st();
+  ptx::tc_fence_before();
+  __syncwarp();
+}
+
+// What warp 2 says about a tile.
 struct Info {
   uint32_t mask[2];                         // keys that count
   uint32_t bad[2];                          // keys of pages that do not exist
-  int page[4];                              // of the tile's pieces; -1: nothing to copy
+  int page[4], in[4];                       // page and place of the tile's pieces; page -1: nothing to copy
 };
 
 template <int FORMAT, int DIM>
 __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __grid_constant__ Args p) {
   constexpr bool CODES = FORMAT != PI05_CACHE_BF16;
-  constexpr int UNITS = units(FORMAT, DIM), UNIT = unit_bytes(DIM), RAW = raw_units(FORMAT, DIM), RAW_UNIT = TILE * DIM, BLOCKS = DIM / 64;
+  constexpr int UNITS = units(FORMAT, DIM), UNIT = unit_bytes(DIM), RAW = CODES ? raw_units(FORMAT, DIM) : 1, RAW_UNIT = TILE * DIM, BLOCKS = DIM / 64;
   constexpr bool OVER = DIM == 256;         // P in place of S
-  constexpr int TM_O = 0, TM_Q = DIM, TM_S = DIM + DIM / 2, TM_P = OVER ? TM_S : TM_S + 2 * TILE, P_STEP = OVER ? TILE : TILE / 2;
+  // S is ahead of P V by LOOK tiles; where there is room in tensor memory the next segment's queries have columns of their own
+  constexpr int LOOK = OVER ? 1 : 2, S_BUFS = LOOK + 1, Q_BUFS = OVER ? 1 : 2;
+  constexpr int TM_O = 0, TM_Q = DIM, TM_S = TM_Q + Q_BUFS * DIM / 2, TM_P = OVER ? TM_S : TM_S + S_BUFS * TILE, P_STEP = OVER ? TILE : TILE / 2;
+  static_assert(TM_P + 2 * P_STEP <= 512, "tensor memory");
   constexpr int TM_COLS = 512;
+  constexpr int TOKEN = 1, END = 9;         // named barriers of a pair of softmax warps: reference handed on (by group), end of a segment
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * INFO + INFO + 2 * UNITS + 2 * (RAW ? RAW : 1) + 1 + 8];
+  __shared__ uint64_t bars[4 * INFO + 2 * UNITS + 2 * RAW + Q_BUFS + 2 * S_BUFS + 5];
   __shared__ Info s_info[INFO];
+  __shared__ float s_vlog[INFO];            // log2 of the largest scale of a tile's values
+  __shared__ uint32_t s_bad[INFO][2];       // Info::bad and the keys whose value's scale is not a number
+  __shared__ float s_ref[2][ROWS];          // the rows' references, by segment
+  __shared__ float2 s_ml[2][2][ROWS];       // at its end: the groups' references and sums
+  __shared__ Segment s_seg[threads(FORMAT) / 32], s_ahead[8];      // a warp's segment; a softmax warp's next one
+  __shared__ Walk s_walk;
+  __shared__ __align__(16) float s_ones[CODES ? TILE : 1];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t ring = ptx::smem_u32(smem), raw = ring + UNITS * UNIT, scales = raw + RAW * RAW_UNIT;
-  long long* sums = reinterpret_cast<long long*>(smem + UNITS * UNIT + RAW * RAW_UNIT + scale_bytes(FORMAT));
-  const float* s_scales = reinterpret_cast<const float*>(smem + UNITS * UNIT + RAW * RAW_UNIT);
+  constexpr int AT_SCALES = UNITS * UNIT + (CODES ? RAW * RAW_UNIT : 0), AT_SUMS = AT_SCALES + scale_bytes(FORMAT);
+  const uint32_t ring = ptx::smem_u32(smem), raw = ring + UNITS * UNIT, scales = ring + AT_SCALES;
+  int* sums = reinterpret_cast<int*>(smem + AT_SUMS);
+  int* lengths = sums + MAX_BATCH + 1;
+  const float* s_scales = reinterpret_cast<const float*>(smem + AT_SCALES);
   uint32_t bar = ptx::smem_u32(bars);
   auto take = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
-  const uint32_t info_full = take(INFO), info_empty = take(INFO), scale_full = take(INFO), kv_full = take(UNITS), kv_empty = take(UNITS),
-                 raw_full = take(RAW ? RAW : 1), raw_empty = take(RAW ? RAW : 1), q_full = take(1), s_full = take(2), s_free = take(2), p_full = take(2), pv_done = take(2);
+  const uint32_t info_full = take(INFO), info_empty = take(INFO), scale_full = take(INFO), vlog_full = take(INFO), kv_full = take(UNITS),
+                 kv_empty = take(UNITS), raw_full = take(RAW), raw_empty = take(RAW), q_full = take(Q_BUFS), o_free = take(1),
+                 s_full = take(S_BUFS), s_free = take(S_BUFS), p_full = take(2), pv_done = take(2);
   const bool leader = ptx::elect_one();
+#define WAIT(BAR, PARITY, KIND) wait(p, BAR, PARITY, KIND)
 
+  if (CODES && tid < TILE) s_ones[tid] = 1.f;
   if (warp == 0) {
     auto init = [&](uint32_t b, int n, int count) { for (int i = lane; i < n; i += 32) ptx::mbar_init(b + 8 * i, count); };
-    init(info_full, INFO, 1); init(info_empty, INFO, 5); init(scale_full, INFO, 1);
-    init(kv_full, UNITS, CODES ? 8 : 1); init(kv_empty, UNITS, 1); init(raw_full, RAW ? RAW : 1, 1); init(raw_empty, RAW ? RAW : 1, 8);
-    init(q_full, 1, 4); init(s_full, 2, 1); init(s_free, 2, 4); init(p_full, 2, 4); init(pv_done, 2, 1);
+    init(info_full, INFO, 1); init(info_empty, INFO, CODES ? 6 : 5); init(scale_full, INFO, 1); init(vlog_full, INFO, 1);
+    init(kv_full, UNITS, CODES ? 4 : 1); init(kv_empty, UNITS, 1); init(raw_full, RAW, 1); init(raw_empty, RAW, 4);
+    init(q_full, Q_BUFS, 4); init(o_free, 1, 8); init(s_full, S_BUFS, 1); init(s_free, S_BUFS, 4); init(p_full, 2, 4); init(pv_done, 2, 1);
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_shared();
     if (leader) { ptx::prefetch_tensormap(&p.k); ptx::prefetch_tensormap(&p.v); }
@@ -216,304 +314,421 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   } else if (warp == 2) {
     // units of the sequences, added up
     ptx::grid_dep_wait();
-    long long before = 0;
+    int before = 0;
     if (lane == 0) sums[0] = 0;
     for (int b0 = 0; b0 < p.s.batch; b0 += 32) {
       const int b = b0 + lane;
-      long long cost = 0;
+      int cost = 0;
       if (b < p.s.batch) {
         const int n = own_length(p, b);
         if (blockIdx.x == 0 && p.s.table && __ldcg(p.s.lengths + b) != n) cache::report(p.c.status, cache::BAD_POSITION, b);
+        lengths[b] = n;
         const int tiles = (p.joined ? p.p_tiles : 0) + (n + TILE - 1) / TILE;
-        cost = tiles ? (long long)(OVERHEAD + tiles) * p.b_tiles : 0;
+        cost = tiles ? (OVERHEAD + tiles) * p.b_tiles : 0;
       }
       for (int d = 1; d < 32; d <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, cost, d);
+        const int up = __shfl_up_sync(0xffffffffu, cost, d);
         if (lane >= d) cost += up;
       }
       if (b < p.s.batch) sums[b + 1] = before + cost;
       before += __shfl_sync(0xffffffffu, cost, 31);
     }
+    __syncwarp();
+    if (lane == 0) s_walk.set(p, sums);
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   ptx::grid_dep_launch();
   const uint32_t tmem = s_tmem;
-  Walk walk;
-  walk.set(p, sums, blockIdx.x);
+  const Walk& walk = s_walk;
   if (blockIdx.x == 0) {
     for (int b = tid; b <= p.s.batch; b += blockDim.x) p.plan[2 + b] = sums[b];
     if (tid == 0) { p.plan[0] = walk.units; p.plan[1] = walk.ctas; }
   }
-  // Where the keys and values of a segment's tile i of n stand among the segment's units: K0, K1, V0, K2, V1, .., K(n-1), V(n-2), V(n-1).
-  auto k_unit = [](int i) { return i ? 2 * i - 1 : 0; };
-  auto v_unit = [](int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; };
+  // Where the keys and values of a segment's tile i of n stand among the segment's units, which is the order of their use: LOOK = 1: K0, K1, V0,
+  // K2, V1, .., V(n-1); 2: K0, K1, K2, V0, K3, V1, .., V(n-2), V(n-1).  And what unit u is.
+  auto k_unit = [](int i) { return i < LOOK ? i : 2 * i - LOOK; };
+  auto v_unit = [](int i, int n) { return i < n - LOOK ? 2 * i + 1 + LOOK : n + i; };
+  auto what = [](int u, int n, bool& is_v) {
+    if (u < LOOK && u < n) { is_v = false; return u; }
+    if (u >= 2 * n - LOOK) { is_v = true; return u - n; }
+    is_v = (u + LOOK) & 1;
+    return is_v ? (u - 1 - LOOK) >> 1 : (u + LOOK) >> 1;
+  };
   bool ok = true;
-  Segment g;
+  const Segment& g = s_seg[warp];
+  int at_unit = walk.begin(blockIdx.x);
+#define NEXT ((at_unit = next_segment(p, walk, at_unit, &s_seg[warp])) >= 0)
 
-  if (warp == 0) {
-    // ---- copies
-    uint32_t unit = 0, tile = 0;            // of all segments
-    ptx::grid_dep_wait();
-    while (ok && walk.next(p, g)) {
-      auto copy = [&](int i, bool is_v) {
-        const uint32_t n = tile + i, slot = n % INFO;
-        if (!is_v) ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
-        if (!ok) return;
-        const Info& info = s_info[slot];
-        const int pieces = TILE / p.piece;
-        int page[4], there = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { page[j] = j < pieces ? info.page[j] : -1; there += page[j] >= 0; }
-        constexpr int RING = CODES ? (RAW ? RAW : 1) : UNITS;
-        const uint32_t full = CODES ? raw_full : kv_full, empty = CODES ? raw_empty : kv_empty, base = CODES ? raw : ring;
-        const uint32_t at = unit % RING, round = unit / RING;
-        ++unit;
-        if (round) ok = ptx::wait_bar(p.c.status + 2, p.limit, empty + 8 * at, (round - 1) & 1, CODES ? WAIT_RAW_EMPTY : WAIT_KV_EMPTY);
-        if (!ok) return;
-        const uint32_t key = (uint32_t)(!g.batch && g.first + i >= (p.joined ? p.p_tiles : 0) ? g.first + i - (p.joined ? p.p_tiles : 0) : g.first + i) * TILE;
-        if (leader) {
-          const uint32_t bar = full + 8 * at, dst = base + at * (CODES ? RAW_UNIT : UNIT);
+  if (warp < 4) {
+    if (warp == 0) {
+      // ---- copies, a lane each
+      uint32_t unit = 0, tile = 0;            // of all segments
+      const int pieces = TILE / p.piece, copies = CODES || p.piece == TILE ? pieces : pieces * BLOCKS, j = lane % pieces, blk = lane / pieces;
+      ptx::grid_dep_wait();
+      while (ok && NEXT) {
+#pragma unroll 1
+        for (int u = 0; u < 2 * g.n && ok; ++u, ++unit) {
+          bool is_v;
+          const uint32_t n = tile + what(u, g.n, is_v), slot = n % INFO;
+          if (!is_v) ok = WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
+          constexpr int RING = CODES ? RAW : UNITS;
+          const uint32_t at = unit % RING, round = unit / RING, full = (CODES ? raw_full : kv_full) + 8 * at;
+          if (ok && round) ok = WAIT((CODES ? raw_empty : kv_empty) + 8 * at, (round - 1) & 1, CODES ? WAIT_RAW_EMPTY : WAIT_KV_EMPTY);
+          if (!ok) break;
+          const int page = s_info[slot].page[j], in = s_info[slot].in[j];
+          const int there = __popc(__ballot_sync(0xffffffffu, lane < pieces && page >= 0));
+          if (leader) {
+            ptx::mbar_expect_tx(full, there * p.piece * DIM * (CODES ? 1 : 2));
+            if (CODES && !is_v) ptx::mbar_expect_tx(scale_full + 8 * slot, there * p.piece * 8);
+          }
+          __syncwarp();
           const CUtensorMap* map = is_v ? &p.v : &p.k;
-          ptx::mbar_expect_tx(bar, there * p.piece * DIM * (CODES ? 1 : 2));
-          if (CODES && !is_v) ptx::mbar_expect_tx(scale_full + 8 * slot, there * p.piece * 8);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (page[j] < 0) continue;
-            const int in = (int)((key + j * p.piece) % (unsigned)p.c.page_tokens);
-            if constexpr (CODES) {
-              ptx::tma_load_4d(dst + j * p.piece * DIM, map, bar, 0, in, g.h, page[j]);
-              if (!is_v) {
-                const long long sc = (((long long)page[j] * p.c.layers + p.s.layer) * p.c.kv_heads + g.h) * p.c.page_tokens + in;
-                const uint32_t sd = scales + (slot * 2 * TILE + j * p.piece) * 4;
-                bulk_load(sd, p.c.k_scale + sc, p.piece * 4, scale_full + 8 * slot);
-                bulk_load(sd + TILE * 4, p.c.v_scale + sc, p.piece * 4, scale_full + 8 * slot);
-              }
-            } else if (p.whole) {
-              ptx::tma_load_5d(dst, map, bar, 0, in, 0, g.h, page[j]);
-            } else {
-#pragma unroll 1
-              for (int blk = 0; blk < BLOCKS; ++blk) ptx::tma_load_5d(dst + blk * TILE * 128 + j * p.piece * 128, map, bar, 0, in, blk, g.h, page[j]);
+          if constexpr (CODES) {
+            const uint32_t dst = raw + at * RAW_UNIT;
+            if (lane < pieces && page >= 0) ptx::tma_load_4d(dst + j * p.piece * DIM, map, full, 0, in, g.h, page);
+            __syncwarp();
+            if (!is_v && lane < 2 * pieces && page >= 0) {           // a piece's scales: of the keys, of the values
+              const long long sc = (((long long)page * p.c.layers + p.s.layer) * p.c.kv_heads + g.h) * p.c.page_tokens + in;
+              bulk_load(scales + ((slot * 2 + blk) * TILE + j * p.piece) * 4, (blk ? p.c.v_scale : p.c.k_scale) + sc, p.piece * 4, scale_full + 8 * slot);
             }
+          } else {
+            const uint32_t dst = ring + at * UNIT;
+            if (lane < copies && page >= 0) ptx::tma_load_5d(dst + blk * TILE * 128 + j * p.piece * 128, map, full, 0, in, blk, g.h, page);
           }
-          if (is_v) ptx::mbar_arrive(info_empty + 8 * slot);
-        }
-        __syncwarp();
-      };
-      copy(0, false);
-      for (int i = 1; i < g.n && ok; ++i) { copy(i, false); copy(i - 1, true); }
-      copy(g.n - 1, true);
-      tile += g.n;
-    }
-  } else if (warp == 1) {
-    // ---- MMAs
-    const uint32_t on = leader ? 1u : 0u;
-    const uint32_t idesc_s = ptx::umma_idesc_bf16(ROWS, TILE), idesc_o = ptx::umma_idesc_bf16(ROWS, DIM) | ptx::UMMA_B_MN_MAJOR;
-    const uint32_t kdesc = (uint32_t)ptx::umma_smem_desc(ring), vdesc = (uint32_t)ptx::umma_smem_desc_mn(ring, TILE * 128);
-    uint32_t unit = 0, tile = 0, seg = 0;
-    while (ok && walk.next(p, g)) {
-      ok = ptx::wait_bar(p.c.status + 2, p.limit, q_full, seg & 1, WAIT_Q);
-      ptx::tc_fence_after();
-      ++seg;
-      auto scores = [&](int i) {
-        const uint32_t n = tile + i, buf = n & 1, u = unit + k_unit(i), at = u % UNITS;
-        if (n > 1) ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, (OVER ? pv_done : s_free) + 8 * buf, ((n >> 1) - 1) & 1, OVER ? WAIT_PV : WAIT_S_FREE);
-        ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const uint32_t kd = kdesc + at * (UNIT >> 4);
-#pragma unroll
-        for (int j = 0; j < DIM / 16; ++j)
-          umma_ts(tmem + TM_S + buf * TILE, tmem + TM_Q + 8 * j, kd + (j >> 2) * (TILE * 128 >> 4) + (j & 3) * 2, idesc_s, j ? 1u : 0u, on);
-        if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(s_full + 8 * buf); }
-        __syncwarp();
-      };
-      auto products = [&](int i) {
-        const uint32_t n = tile + i, buf = n & 1, u = unit + v_unit(i, g.n), at = u % UNITS;
-        ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
-        ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, p_full + 8 * buf, (n >> 1) & 1, WAIT_P);
-        if (!ok) return;
-        ptx::tc_fence_after();
-        const uint32_t vd = vdesc + at * (UNIT >> 4);
-#pragma unroll
-        for (int j = 0; j < TILE / 16; ++j)
-          umma_ts(tmem + TM_O, tmem + TM_P + buf * P_STEP + 8 * j, vd + j * (16 * 128 >> 4), idesc_o, i || j ? 1u : 0u, on);
-        if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(pv_done + 8 * buf); }
-        __syncwarp();
-      };
-      if (ok) scores(0);
-      for (int i = 1; i < g.n && ok; ++i) { scores(i); products(i - 1); }
-      if (ok) products(g.n - 1);
-      unit += 2 * g.n;
-      tile += g.n;
-    }
-  } else if (warp < 4) {
-    // ---- pages and masks, every second tile each
-    uint32_t tile = 0;
-    while (ok && walk.next(p, g)) {
-      const int p_tiles = g.batch || p.joined ? p.p_tiles : 0, length = g.batch ? 0 : own_length(p, g.b);
-      for (int i = 0; i < g.n && ok; ++i) {
-        const uint32_t n = tile + i, slot = n % INFO;
-        if ((n & 1) != (uint32_t)(warp & 1)) continue;
-        const bool own = g.first + i >= p_tiles;
-        const uint32_t key = (uint32_t)(own ? g.first + i - p_tiles : g.first + i) * TILE;
-        const uint32_t end = own ? length : p.s.prefix_tokens;
-        const int* table = own ? p.s.table + (long long)g.b * p.s.table_stride : p.s.prefix_table;
-        const uint32_t first = key + lane * p.piece;
-        int page = -1;
-        bool bad = false;
-        if (lane < TILE / p.piece && first < end) {
-          page = __ldcg(table + first / (unsigned)p.c.page_tokens);
-          bad = page < 0 || page >= p.c.pages;
-          if (bad) { page = -1; cache::report(p.c.status, cache::BAD_PAGE, own ? g.b : -1); }
-        }
-        bool c0 = key + lane < end, c1 = key + 32 + lane < end;
-        if (!own && p.s.prefix_valid) {
-          c0 = c0 && __ldcg(p.s.prefix_valid + key + lane);
-          c1 = c1 && __ldcg(p.s.prefix_valid + key + 32 + lane);
-        }
-        const unsigned lost = __ballot_sync(0xffffffffu, bad);
-        const bool b0 = lost >> (lane / p.piece) & 1, b1 = lost >> ((lane + 32) / p.piece) & 1;
-        const unsigned m0 = __ballot_sync(0xffffffffu, c0), m1 = __ballot_sync(0xffffffffu, c1), l0 = __ballot_sync(0xffffffffu, b0 && c0),
-                       l1 = __ballot_sync(0xffffffffu, b1 && c1);
-        if (n >= INFO) ok = ptx::wait_bar(p.c.status + 2, p.limit, info_empty + 8 * slot, (n / INFO - 1) & 1, WAIT_INFO_EMPTY);
-        if (!ok) break;
-        Info& info = s_info[slot];
-        if (lane < 4) info.page[lane] = page;
-        if (lane == 0) { info.mask[0] = m0; info.mask[1] = m1; info.bad[0] = l0; info.bad[1] = l1; }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(info_full + 8 * slot);
-        __syncwarp();
-      }
-      tile += g.n;
-    }
-  } else if (warp < 8) {
-    // ---- softmax: thread = query row.  A wait that gave up lets the rest run through, with NaN as the result
-    const int quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t unit = 0, tile = 0;
-    const uint4* q = nullptr;
-    int sees = 0;                           // own tokens that the row sees
-    bool mine = false;
-    int b = 0, t = 0, head = 0;
-    ptx::grid_dep_wait();
-    while (walk.next(p, g)) {
-      mine = row_of(p, g, row, b, t, head);
-      q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.s.q) + b * p.s.q_batch_stride + t * p.s.q_token_stride + head * p.s.q_head_stride);
-#pragma unroll 1
-      for (int c = 0; c < DIM / 64; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint4 x = mine ? __ldcg(q + c * 8 + j) : make_uint4(0u, 0u, 0u, 0u);
-          w[4 * j] = x.x; w[4 * j + 1] = x.y; w[4 * j + 2] = x.z; w[4 * j + 3] = x.w;
-        }
-        tmem_st_32x32(lanes + TM_Q + 32 * c, w);
-      }
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(q_full);
-      __syncwarp();
-      const int p_tiles = g.batch || p.joined ? p.p_tiles : 0, length = g.batch ? 0 : own_length(p, g.b);
-      sees = p.s.causal ? length - p.s.tokens + t + 1 : length;
-      float m = -INFINITY, l = 0.f;         // reference (of exponents to the base 2) and sum
-#pragma unroll 1
-      for (int i = 0; i < g.n; ++i) {
-        const uint32_t n = tile + i, buf = n & 1, slot = n % INFO;
-        ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
-        if (CODES) ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, scale_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
-        const uint32_t mask0 = s_info[slot].mask[0], mask1 = s_info[slot].mask[1], bad0 = s_info[slot].bad[0], bad1 = s_info[slot].bad[1];
-        uint32_t k0 = mask0, k1 = mask1;    // keys that count for this row
-        if (g.first + i >= p_tiles) {
-          const long long left = sees - (long long)(g.first + i - p_tiles) * TILE;
-          k0 &= left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-          k1 &= left >= 64 ? 0xffffffffu : left > 32 ? (1u << (left - 32)) - 1u : 0u;
-        }
-        const bool special = __any_sync(0xffffffffu, (k0 & k1) != 0xffffffffu || (bad0 | bad1));
-        ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, s_full + 8 * buf, (n >> 1) & 1, WAIT_S);
-        ptx::tc_fence_after();
-        float x[64];
-        ptx::tmem_ld_32x32(lanes + TM_S + buf * TILE, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-        ptx::tmem_ld_32x32(lanes + TM_S + buf * TILE + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
-        ptx::tmem_wait_ld();
-        if (!OVER) {
-          ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(s_free + 8 * buf);
+          if (is_v && leader) ptx::mbar_arrive(info_empty + 8 * slot);
           __syncwarp();
         }
-        const float4* ks = reinterpret_cast<const float4*>(s_scales + slot * 2 * TILE);
-        if (CODES) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float4 f = ks[j];
-            x[4 * j] *= f.x; x[4 * j + 1] *= f.y; x[4 * j + 2] *= f.z; x[4 * j + 3] *= f.w;
-          }
-        }
-        if (special) {
-#pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            if (!((j < 32 ? k0 : k1) >> (j & 31) & 1)) x[j] = -INFINITY;
-            else if ((j < 32 ? bad0 : bad1) >> (j & 31) & 1) x[j] = __uint_as_float(0x7fffffffu);
-          }
-        }
-        float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int j = 4; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], x[j]);
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c_log2;
-        if (i == 0) {
-          m = high;
-        } else {
-          const bool move = high > m + RESCALE;
-          if (__any_sync(0xffffffffu, move)) {
-            const float f = move ? ptx::ex2_approx(m - high) : 1.f;
-            if (move) m = high;
-            l *= f;
-            ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, pv_done + 8 * (buf ^ 1), ((n - 1) >> 1) & 1, WAIT_PV);
+        tile += g.n;
+      }
+    } else if (warp == 1) {
+      // ---- MMAs
+      const uint32_t on = leader ? 1u : 0u;
+      const uint32_t idesc_s = ptx::umma_idesc_bf16(ROWS, TILE);
+      const uint32_t idesc_o = (ptx::umma_idesc_bf16(ROWS, DIM) & (CODES ? ~((1u << 7) | (1u << 10)) : ~0u)) | ptx::UMMA_B_MN_MAJOR;     // (FP16 is type 0)
+      const uint32_t kdesc = (uint32_t)ptx::umma_smem_desc(ring), vdesc = (uint32_t)ptx::umma_smem_desc_mn(ring, TILE * 128);
+      uint32_t unit = 0, tile = 0, seg = 0;
+      while (ok && NEXT) {
+        ok = WAIT(q_full + 8 * (seg % Q_BUFS), (seg / Q_BUFS) & 1, WAIT_Q);
+        ptx::tc_fence_after();
+        const uint32_t q = tmem + TM_Q + seg % Q_BUFS * (DIM / 2);
+#pragma unroll 1
+        for (int i = 0; i < g.n + LOOK && ok; ++i) {
+          if (i < g.n) {
+            const uint32_t n = tile + i, buf = n % S_BUFS, u = unit + k_unit(i), at = u % UNITS;
+            if (OVER && n > 1) ok = WAIT(pv_done + 8 * buf, ((n >> 1) - 1) & 1, WAIT_PV);
+            if (!OVER && n >= S_BUFS) ok = WAIT(s_free + 8 * buf, (n / S_BUFS - 1) & 1, WAIT_S_FREE);
+            if (ok) ok = WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
+            if (!ok) break;
             ptx::tc_fence_after();
+            const uint32_t kd = kdesc + at * (UNIT >> 4);
+#pragma unroll
+            for (int j = 0; j < BLOCKS; ++j) umma_ts4<2>(tmem + TM_S + buf * TILE, q + 32 * j, kd + j * (TILE * 128 >> 4), idesc_s, j ? 1u : 0u, on);
+            if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(s_full + 8 * buf); }
+            __syncwarp();
+          }
+          if (i >= LOOK) {
+            const uint32_t n = tile + i - LOOK, buf = n & 1, u = unit + v_unit(i - LOOK, g.n), at = u % UNITS;
+            if (i == LOOK && seg) ok = WAIT(o_free, (seg - 1) & 1, WAIT_O_FREE);
+            if (ok) ok = WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
+            if (ok) ok = WAIT(p_full + 8 * buf, (n >> 1) & 1, WAIT_P);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t vd = vdesc + at * (UNIT >> 4);
+            umma_ts4<(16 * 128 >> 4)>(tmem + TM_O, tmem + TM_P + buf * P_STEP, vd, idesc_o, i > LOOK ? 1u : 0u, on);
+            if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(pv_done + 8 * buf); }
+            __syncwarp();
+          }
+        }
+        unit += 2 * g.n;
+        tile += g.n;
+        ++seg;
+      }
+    } else if (warp == 2) {
+      // ---- pages and masks, eight tiles at a time: a lane looks up a piece
+      uint32_t tile = 0;
+      const int pieces = TILE / p.piece;
+      while (ok && NEXT) {
+        const int p_tiles = g.batch || p.joined ? p.p_tiles : 0;
+        const uint32_t length = g.batch ? 0 : lengths[g.b];
 #pragma unroll 1
-            for (int c = 0; c < DIM; c += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld_32x32(lanes + TM_O + c, o);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st_32x32(lanes + TM_O + c, o);
+        for (int i0 = 0; i0 < g.n && ok; i0 += BATCH) {
+          // this lane's piece of tile i0 + lane / pieces
+          int page = -1, in = 0;
+          bool bad = false;
+          {
+            const int i = g.first + i0 + lane / pieces;
+            const bool own = i >= p_tiles;
+            const uint32_t first = (uint32_t)(own ? i - p_tiles : i) * TILE + lane % pieces * p.piece, end = own ? length : (uint32_t)p.s.prefix_tokens;
+            if (lane < BATCH * pieces && i < g.first + g.n && first < end) {
+              const uint32_t lp = first / (uint32_t)p.c.page_tokens;
+              in = (int)(first - lp * (uint32_t)p.c.page_tokens);
+              page = __ldcg((own ? p.s.table + (long long)g.b * p.s.table_stride : p.s.prefix_table) + lp);
+              bad = page < 0 || page >= p.c.pages;
+              if (bad) { page = -1; cache::report(p.c.status, cache::BAD_PAGE, own ? g.b : -1); }
             }
-            ptx::tmem_wait_st();
+          }
+          const unsigned gone = __ballot_sync(0xffffffffu, bad);
+          uint32_t m0 = 0, m1 = 0;            // lane k: keys of tile i0 + k
+          const bool masked = p.s.prefix_valid && g.first + i0 < p_tiles;
+          uint8_t valid[2 * BATCH];           // (all on their way before the first is looked at)
+#pragma unroll
+          for (int k = 0; k < 2 * BATCH; ++k) {
+            const int i = g.first + i0 + k / 2;
+            const uint32_t key = (uint32_t)i * TILE + (k & 1) * 32 + lane;
+            valid[k] = 1;
+            if (masked && i < p_tiles && key < (uint32_t)p.s.prefix_tokens) valid[k] = __ldcg(p.s.prefix_valid + key);
+          }
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            const int i = g.first + i0 + k;
+            const bool own = i >= p_tiles;
+            const uint32_t key = (uint32_t)(own ? i - p_tiles : i) * TILE + lane, end = i0 + k >= g.n ? 0u : own ? length : (uint32_t)p.s.prefix_tokens;
+            const unsigned w0 = __ballot_sync(0xffffffffu, key < end && valid[2 * k]), w1 = __ballot_sync(0xffffffffu, key + 32 < end && valid[2 * k + 1]);
+            if (lane == k) { m0 = w0; m1 = w1; }
+          }
+#pragma unroll 1
+          for (int k = 0; k < BATCH && i0 + k < g.n && ok; ++k) {
+            const uint32_t n = tile + i0 + k, slot = n % INFO;
+            if (n >= INFO) ok = WAIT(info_empty + 8 * slot, (n / INFO - 1) & 1, WAIT_INFO_EMPTY);
+            if (!ok) break;
+            Info& info = s_info[slot];
+            const int j = lane - k * pieces;
+            if (j >= 0 && j < pieces) { info.page[j] = page; info.in[j] = in; }
+            if (lane == k) {
+              uint32_t b0 = 0, b1 = 0;
+              for (int q = 0; q < pieces; ++q)
+                if (gone >> (k * pieces + q) & 1) {
+                  const unsigned long long keys = (p.piece == 64 ? ~0ull : (1ull << p.piece) - 1) << (q * p.piece);
+                  b0 |= (uint32_t)keys;
+                  b1 |= (uint32_t)(keys >> 32);
+                }
+              info.mask[0] = m0; info.mask[1] = m1; info.bad[0] = b0 & m0; info.bad[1] = b1 & m1;
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(info_full + 8 * slot);
+            __syncwarp();
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t pk[32];
-#pragma unroll
-        for (int j = 0; j < 64; j += 4) {
-          float e[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) { e[k] = ptx::ex2_approx(fmaf(x[j + k], p.c_log2, -ref)); sum[k] += e[k]; }
-          if (CODES) {
-            const float4 f = ks[16 + j / 4];
-            e[0] *= f.x; e[1] *= f.y; e[2] *= f.z; e[3] *= f.w;
-            if (special)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) e[k] = (j < 32 ? k0 : k1) >> ((j + k) & 31) & 1 ? e[k] : 0.f;
+        tile += g.n;
+      }
+    } else if (warp == 3) {
+      // ---- the largest scale of a tile's values that count
+      if constexpr (CODES) {
+        uint32_t tile = 0;
+        while (ok && NEXT) {
+#pragma unroll 1
+          for (int i = 0; i < g.n && ok; ++i) {
+            const uint32_t n = tile + i, slot = n % INFO;
+            ok = WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
+            if (ok) ok = WAIT(scale_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
+            if (!ok) break;
+            float* vs = const_cast<float*>(s_scales) + (slot * 2 + 1) * TILE;
+            const Info& info = s_info[slot];
+            const bool c0 = (info.mask[0] & ~info.bad[0]) >> lane & 1, c1 = (info.mask[1] & ~info.bad[1]) >> lane & 1;
+            const float v0 = c0 ? vs[lane] : 0.f, v1 = c1 ? vs[lane + 32] : 0.f;
+            // a scale that does not count is whatever memory holds, and 0 x NaN is NaN: zero in its place, also where it counts and is not a number
+            const bool f0 = fabsf(v0) < INFINITY, f1 = fabsf(v1) < INFINITY;
+            if (!c0 || !f0) vs[lane] = 0.f;
+            if (!c1 || !f1) vs[lane + 32] = 0.f;
+            const unsigned n0 = __ballot_sync(0xffffffffu, !f0), n1 = __ballot_sync(0xffffffffu, !f1);
+            float top = fmaxf(f0 ? v0 : 0.f, f1 ? v1 : 0.f);
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (lane == 0) {
+              s_vlog[slot] = fmaxf(__log2f(top), -92.f) - 7.f;       // (of zeros: sums up to 2^99 a key have room in FP32)  7: see the softmax
+              s_bad[slot][0] = info.bad[0] | n0;
+              s_bad[slot][1] = info.bad[1] | n1;
+              ptx::mbar_arrive(vlog_full + 8 * slot);
+              ptx::mbar_arrive(info_empty + 8 * slot);
+            }
+            __syncwarp();
           }
-          pk[j / 2] = cache::pack2(e[0], e[1]);
-          pk[j / 2 + 1] = cache::pack2(e[2], e[3]);
+          tile += g.n;
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (!OVER && n > 1) {               // the buffer of P is free once the product before the last has read it
-          ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, pv_done + 8 * buf, ((n >> 1) - 1) & 1, WAIT_PV);
+      }
+    }
+  } else if (warp < 12) {
+    // ---- softmax: thread = query row, group = every second tile.  A wait that gave up lets the rest run through, with NaN as the result
+    const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    uint32_t unit = 0, tile = 0, seg = 0;
+    auto load_q = [&](const Segment& s, uint32_t seg) {
+      load_queries<DIM>(p, s, row, lanes + TM_Q + seg % Q_BUFS * (DIM / 2));
+      if (lane == 0) ptx::mbar_arrive(q_full + 8 * (seg % Q_BUFS));
+      __syncwarp();
+    };
+    const int sw = warp - 4;
+    ptx::grid_dep_wait();
+    int at = next_segment(p, walk, walk.begin(blockIdx.x), &s_seg[warp]);
+    bool more = at >= 0;
+    if (more && group == 1) load_q(s_seg[warp], 0);        // (the first tile is the other group's)
+    while (more) {
+      const int par = seg & 1;
+      const Segment& d = par ? s_ahead[sw] : s_seg[warp];
+      Segment& ahead = par ? s_seg[warp] : s_ahead[sw];      // the one after it
+      const int count = d.n;
+      int own;                              // of the segment's first tile: its place among the tiles of own tokens
+      int sees;                             // own tokens that the row sees
+      bool mine, idle;
+      {
+        int b = 0, t = 0, head = 0;
+        mine = row_of(p, d, row, b, t, head);
+        idle = !__any_sync(0xffffffffu, mine);
+        own = d.first - (d.batch || p.joined ? p.p_tiles : 0);
+        const int length = d.batch ? 0 : lengths[d.b];
+        sees = p.s.causal ? length - p.s.tokens + t + 1 : length;
+      }
+      float m = -INFINITY, l = 0.f;         // reference (of exponents to the base 2) and sum
+      at = next_segment(p, walk, at, &ahead);
+      more = at >= 0;
+      if (Q_BUFS == 2 && more && ((tile & 1) ^ group)) load_q(ahead, seg + 1);
+#pragma unroll 1
+      for (int i = (tile & 1) ^ group; i < count; i += 2) {
+        const uint32_t n = tile + i, buf = group, sbuf = n % S_BUFS, slot = n % INFO;
+        ok = ok && WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
+        if (CODES) {
+          ok = ok && WAIT(scale_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
+          ok = ok && WAIT(vlog_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
+        }
+        const uint32_t mask0 = s_info[slot].mask[0], mask1 = s_info[slot].mask[1];
+        const uint32_t bad0 = CODES ? s_bad[slot][0] : s_info[slot].bad[0], bad1 = CODES ? s_bad[slot][1] : s_info[slot].bad[1];
+        uint32_t k0 = mask0, k1 = mask1;    // keys that count for this row
+        if (own + i >= 0) {
+          const int left = sees - (own + i) * TILE;
+          if (left < TILE) {
+            k0 &= left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+            k1 &= left > 32 ? (1u << (left - 32)) - 1u : 0u;
+          }
+        }
+        const bool poison = (k0 & bad0) | (k1 & bad1);     // the row sees a key that does not exist, or a value that is not a number
+        k0 &= ~bad0;
+        k1 &= ~bad1;
+        const bool special = __any_sync(0xffffffffu, (k0 & k1) != 0xffffffffu);
+        ok = ok && WAIT(s_full + 8 * sbuf, (n / S_BUFS) & 1, WAIT_S);
+        ptx::tc_fence_after();
+        const float4* ks = reinterpret_cast<const float4*>(s_scales + slot * 2 * TILE);
+        const uint32_t s_at = lanes + TM_S + sbuf * TILE, p_at = lanes + TM_P + buf * P_STEP;
+        // A tile is read twice, 32 scores at a time: for the row's maximum, then for the probabilities.  (With all 64 in registers
+        // the kernel's code is twice as long, and what its warps execute no longer fits the instruction cache)
+        float high = -INFINITY;
+        if (!idle) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            ptx::tmem_ld_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
+            ptx::tmem_wait_ld();
+            if (CODES) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 f = ks[h * 8 + j / 4];
+                const float2 y = mul2(make_float2(x[j], x[j + 1]), make_float2(f.x, f.y)), z = mul2(make_float2(x[j + 2], x[j + 3]), make_float2(f.z, f.w));
+                x[j] = y.x; x[j + 1] = y.y; x[j + 2] = z.x; x[j + 3] = z.y;
+              }
+            }
+            if (special) {                  // keys that do not count: -infinity, there (scaled) for the second time too
+              const uint32_t k = h ? k1 : k0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = k >> j & 1 ? x[j] : -INFINITY;
+              tmem_st_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
+            }
+            float a = high, b = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              a = fmaxf(fmaxf(a, x[j]), x[j + 1]);
+              b = fmaxf(fmaxf(b, x[j + 2]), x[j + 3]);
+            }
+            high = fmaxf(a, b);
+          }
+          if (special) ptx::tmem_wait_st();
+          high *= p.c_log2;
+          if (CODES) high += s_vlog[slot];  // largest exponent of a probability times its value's scale, or a little more; 7 less: products up to 2^15 at 2^RESCALE
+          bool write = true;
+          if (i == 0) {
+            m = high;
+          } else {
+            ptx::named_bar_sync(TOKEN + 4 * group + quad, 64);
+            const float r = s_ref[par][row];
+            if (r != m) { l *= ptx::ex2_approx(m - r); m = r; }
+            const bool move = high > m + RESCALE;
+            write = __any_sync(0xffffffffu, move);
+            if (write) {
+              const float f = move ? ptx::ex2_approx(m - high) : 1.f;
+              if (move) m = high;
+              l *= f;
+              ok = ok && WAIT(pv_done + 8 * (buf ^ 1), ((n - 1) >> 1) & 1, WAIT_PV);
+              ptx::tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < DIM; c += 16) {
+                uint32_t o[16];
+                ptx::tmem_ld_32x16(lanes + TM_O + c, o);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                ptx::tmem_st_32x8(lanes + TM_O + c, reinterpret_cast<uint32_t(&)[8]>(o[0]));
+                ptx::tmem_st_32x8(lanes + TM_O + c + 8, reinterpret_cast<uint32_t(&)[8]>(o[8]));
+              }
+              ptx::tmem_wait_st();
+            }
+          }
+          if (write) s_ref[par][row] = m;
+          __syncwarp();
+          if (i + 1 < count) ptx::bar_arrive(TOKEN + 4 * (group ^ 1) + quad, 64);
+        }
+        // The buffer of P is free once the product before the last has read it.  (A warp without rows waits as well: it must not report its part of
+        // this tile before the others have reported theirs of that one)
+        if (!OVER && n > 1) {
+          ok = ok && WAIT(pv_done + 8 * buf, ((n >> 1) - 1) & 1, WAIT_PV);
           ptx::tc_fence_after();
         }
-        tmem_st_32x32(lanes + TM_P + buf * P_STEP, pk);
-        ptx::tmem_wait_st();
+        if (!idle) {
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float2 c2 = make_float2(p.c_log2, p.c_log2), r2 = make_float2(-ref, -ref);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float4* scale = special ? reinterpret_cast<const float4*>(s_ones) : ks;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            ptx::tmem_ld_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
+            ptx::tmem_wait_ld();
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              float2 e = make_float2(x[j], x[j + 1]), f = make_float2(x[j + 2], x[j + 3]);
+              if (CODES) {
+                const float4 s = scale[h * 8 + j / 4];
+                e = mul2(e, make_float2(s.x, s.y));
+                f = mul2(f, make_float2(s.z, s.w));
+              }
+              e = ptx::fma2(e, c2, r2);
+              f = ptx::fma2(f, c2, r2);
+              e.x = ptx::ex2_approx(e.x); e.y = ptx::ex2_approx(e.y); f.x = ptx::ex2_approx(f.x); f.y = ptx::ex2_approx(f.y);
+              sum[0] = add2(sum[0], e);
+              sum[1] = add2(sum[1], f);
+              if (CODES) {
+                const float4 s = ks[TILE / 4 + h * 8 + j / 4];
+                e = mul2(e, make_float2(s.x, s.y));
+                f = mul2(f, make_float2(s.z, s.w));
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[j / 2]) : "f"(e.y), "f"(e.x));
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[j / 2 + 1]) : "f"(f.y), "f"(f.x));
+              } else {
+                pk[j / 2] = cache::pack2(e.x, e.y);
+                pk[j / 2 + 1] = cache::pack2(f.x, f.y);
+              }
+            }
+            ptx::tmem_st_32x8(p_at + 16 * h, reinterpret_cast<uint32_t(&)[8]>(pk[0]));
+            ptx::tmem_st_32x8(p_at + 16 * h + 8, reinterpret_cast<uint32_t(&)[8]>(pk[8]));
+          }
+          const float2 both = add2(sum[0], sum[1]);
+          l += both.x + both.y;
+          if (poison) l = __uint_as_float(0x7fffffffu);
+          ptx::tmem_wait_st();
+        }
         if (!CODES && (mask0 & mask1 & ~(bad0 | bad1)) != 0xffffffffu) {
           // values at places that do not count are whatever memory holds, and 0 x NaN is NaN: zeros in their place
-          const uint32_t u = unit + v_unit(i, g.n), at = u % UNITS;
-          ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
+          const uint32_t u = unit + v_unit(i, count), at = u % UNITS;
+          ok = ok && WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
           const uint32_t z0 = ~mask0 | bad0, z1 = ~mask1 | bad1;
           for (int c = row; c < TILE * DIM / 8; c += 128) {
             const int key = c & 63, chunk = c >> 6;
@@ -521,87 +736,116 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           }
           ptx::fence_proxy_async_shared();
         }
-        __syncwarp();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) { ptx::mbar_arrive(p_full + 8 * buf); ptx::mbar_arrive(info_empty + 8 * slot); }
+        if (lane == 0) {
+          if (!OVER) ptx::mbar_arrive(s_free + 8 * sbuf);
+          ptx::mbar_arrive(p_full + 8 * buf);
+          ptx::mbar_arrive(info_empty + 8 * slot);
+        }
         __syncwarp();
       }
-      unit += 2 * g.n;
-      tile += g.n;
-      // ---- the segment's sums
-      ok = ok && ptx::wait_bar(p.c.status + 2, p.limit, pv_done + 8 * ((tile - 1) & 1), ((tile - 1) >> 1) & 1, WAIT_PV);
+      const uint32_t last = tile + count - 1;
+      unit += 2 * count;
+      tile += count;
+      // ---- the next segment's queries, by the group that does not have the last tile, once the last scores are there
+      if (Q_BUFS == 1 && more && (last & 1) != (uint32_t)group) {
+        ok = ok && WAIT(s_full + 8 * (last % S_BUFS), (last / S_BUFS) & 1, WAIT_S);
+        ptx::tc_fence_after();
+        load_q(ahead, seg + 1);
+      }
+      // ---- the segment's sums, half of the columns each
+      if (!idle) {
+        s_ml[par][group][row] = make_float2(m, l);
+        ptx::named_bar_sync(END + quad, 64);
+        const float2 other = s_ml[par][group ^ 1][row];
+        const float r = s_ref[par][row];
+        l = (m == r ? l : l * ptx::ex2_approx(m - r)) + (other.x == r ? other.y : other.y * ptx::ex2_approx(other.x - r));
+        m = r;
+      }
+      ok = ok && WAIT(pv_done + 8 * (last & 1), (last >> 1) & 1, WAIT_PV);
       ptx::tc_fence_after();
       if (!ok) l = __uint_as_float(0x7fffffffu);
-      if (!g.batch && p.joined && g.n == g.tiles) {
-        const float il = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;        // (no key: zeros; NaN stays)
+      if (!idle) {
+        int b = 0, t = 0, head = 0;
+        row_of(p, d, row, b, t, head);
+        const bool direct = !d.batch && p.joined && d.n == d.tiles;
+        const float il = !direct ? 1.f : l == 0.f ? 0.f : 1.0f / l;        // (no key: zeros)
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.s.out) + b * p.s.out_batch_stride + t * p.s.out_token_stride + head * p.s.out_head_stride;
+        const int rows = d.batch ? ROWS : p.b_slot;
+        float* part = (d.batch ? p.a_parts : p.b_parts) + (long long)(blockIdx.x + d.item) * rows * (DIM + 2);
 #pragma unroll 1
-        for (int c = 0; c < DIM; c += 32) {
+        for (int c = group * (DIM / 2); c < (group + 1) * (DIM / 2); c += 32) {
           uint32_t o[32];
           ptx::tmem_ld_32x32(lanes + TM_O + c, o);
           ptx::tmem_wait_ld();
-          if (mine)
+          if (mine && direct) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8)
               *reinterpret_cast<uint4*>(out + c + j) = make_uint4(
                   cache::pack2(__uint_as_float(o[j]) * il, __uint_as_float(o[j + 1]) * il), cache::pack2(__uint_as_float(o[j + 2]) * il, __uint_as_float(o[j + 3]) * il),
                   cache::pack2(__uint_as_float(o[j + 4]) * il, __uint_as_float(o[j + 5]) * il), cache::pack2(__uint_as_float(o[j + 6]) * il, __uint_as_float(o[j + 7]) * il));
-          __syncwarp();
-        }
-        if (mine && p.s.lse) p.s.lse[((long long)b * p.s.tokens + t) * p.s.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      } else {
-        const int rows = g.batch ? ROWS : p.b_slot;
-        float* part = (g.batch ? p.a_parts : p.b_parts) + (long long)(blockIdx.x + g.item) * rows * (DIM + 2);
-#pragma unroll 1
-        for (int c = 0; c < DIM; c += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(lanes + TM_O + c, o);
-          ptx::tmem_wait_ld();
-          if (mine)
+          } else if (mine) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
               __stcg(reinterpret_cast<uint4*>(part) + ((c + j) / 4) * rows + row, make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+          }
           __syncwarp();
         }
-        if (mine) __stcg(reinterpret_cast<float2*>(part + DIM * rows) + row, make_float2(m, l));
+        if (mine && group == 0) {
+          if (!direct) __stcg(reinterpret_cast<float2*>(part + DIM * rows) + row, make_float2(m, l));
+          else if (p.s.lse) p.s.lse[((long long)b * p.s.tokens + t) * p.s.q_heads + head] = l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(l)) * 0.6931471805599453f;
+        }
       }
+      ++seg;
       ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(o_free);
       __syncwarp();
     }
   } else if constexpr (CODES) {
-    // ---- codes to BF16: 16 codes per thread and turn, to two 16-byte chunks of the swizzled unit.  Eight neighbouring lanes take 64 bytes
-    // of an even row and the other 64 of the odd one, so that neither the loads nor the stores share banks
-    const int w = warp - 8, odd = lane >> 2 & 1, chunk = lane & 3, high = lane >> 3;
+    // ---- codes to 16 bits, the two groups in turn: 16 codes per thread and turn, to two 16-byte chunks of the swizzled unit.  Eight
+    // neighbouring lanes take 64 bytes of an even row and the other 64 of the odd one, so that neither the loads nor the stores share banks
+    const int group = (warp - 12) >> 2, w = warp & 3, odd = lane >> 2 & 1, chunk = lane & 3, high = lane >> 3;
     const int blk = BLOCKS == 4 ? high ^ odd : BLOCKS == 2 ? (high & 1) ^ odd : 0;
     constexpr int AT_ONCE = 8 / BLOCKS;     // rows of a warp's turn
     const int first = odd + (BLOCKS == 4 ? 0 : BLOCKS == 2 ? (high >> 1) * 2 : high * 2);
     uint32_t unit = 0;
-    while (ok && walk.next(p, g)) {
-      for (int i = 0; i < 2 * g.n && ok; ++i, ++unit) {
-        const uint32_t from = unit % RAW, to = unit % UNITS;
-        ok = ptx::wait_bar(p.c.status + 2, p.limit, raw_full + 8 * from, (unit / RAW) & 1, WAIT_RAW_FULL);
-        if (ok && unit >= UNITS) ok = ptx::wait_bar(p.c.status + 2, p.limit, kv_empty + 8 * to, (unit / UNITS - 1) & 1, WAIT_KV_EMPTY);
+    while (ok && NEXT) {
+#pragma unroll 1
+      for (int u = (unit & 1) ^ group; u < 2 * g.n && ok; u += 2) {
+        bool is_v;
+        what(u, g.n, is_v);
+        const uint32_t n = unit + u, from = n % RAW, to = n % UNITS;
+        ok = WAIT(raw_full + 8 * from, (n / RAW) & 1, WAIT_RAW_FULL);
+        if (ok && n >= UNITS) ok = WAIT(kv_empty + 8 * to, (n / UNITS - 1) & 1, WAIT_KV_EMPTY);
         if (!ok) break;
-        constexpr int TURNS = TILE / AT_ONCE / 8;
+        constexpr int TURNS = TILE / AT_ONCE / 4;
         uint4 x[TURNS];
 #pragma unroll
-        for (int j = 0; j < TURNS; ++j) x[j] = ptx::ld_shared_v4(raw + from * RAW_UNIT + ((j * 8 + w) * AT_ONCE + first) * DIM + blk * 64 + chunk * 16);
+        for (int j = 0; j < TURNS; ++j) x[j] = ptx::ld_shared_v4(raw + from * RAW_UNIT + ((j * 4 + w) * AT_ONCE + first) * DIM + blk * 64 + chunk * 16);
+        auto turn = [&](auto value) {
 #pragma unroll
-        for (int j = 0; j < TURNS; ++j) {
-          const int r = (j * 8 + w) * AT_ONCE + first;
-          const uint2 a = cache::quad<FORMAT>(x[j].x), c = cache::quad<FORMAT>(x[j].y), d = cache::quad<FORMAT>(x[j].z), e = cache::quad<FORMAT>(x[j].w);
-          const uint32_t line = ring + to * UNIT + blk * (TILE * 128) + r * 128;
-          ptx::st_shared_v4(line + (((2 * chunk) ^ (r & 7)) << 4), a.x, a.y, c.x, c.y);
-          ptx::st_shared_v4(line + (((2 * chunk + 1) ^ (r & 7)) << 4), d.x, d.y, e.x, e.y);
-        }
+          for (int j = 0; j < TURNS; ++j) {
+            const int r = (j * 4 + w) * AT_ONCE + first;
+            const uint2 a = value(x[j].x), c = value(x[j].y), d = value(x[j].z), e = value(x[j].w);
+            const uint32_t line = ring + to * UNIT + blk * (TILE * 128) + r * 128;
+            ptx::st_shared_v4(line + (((2 * chunk) ^ (r & 7)) << 4), a.x, a.y, c.x, c.y);
+            ptx::st_shared_v4(line + (((2 * chunk + 1) ^ (r & 7)) << 4), d.x, d.y, e.x, e.y);
+          }
+        };
+        if (is_v) turn([](uint32_t c) { return cache::quad_half<FORMAT>(c); });
+        else turn([](uint32_t c) { return cache::quad<FORMAT>(c); });
         ptx::fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) { ptx::mbar_arrive(kv_full + 8 * to); ptx::mbar_arrive(raw_empty + 8 * from); }
         __syncwarp();
       }
+      unit += 2 * g.n;
     }
   }
+#undef WAIT
+#undef NEXT
   ptx::tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -619,33 +863,31 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Ar
   ptx::grid_dep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, share = warp % split;
   const int flat = p.s.batch * p.s.tokens * p.group, groups = (flat + 7) / 8;
-  const long long work = (long long)blockIdx.x * (8 / split) + warp / split;
-  const int column = (int)(work % (DIM / 16)) * 4 + (lane & 3);          // of four dims
-  const long long hg = work / (DIM / 16);
-  const int h = (int)(hg / groups), f = (int)(hg % groups) * 8 + row;
+  const int work = blockIdx.x * (8 / split) + warp / split, hg = work / (DIM / 16);
+  const int column = (work & (DIM / 16 - 1)) * 4 + (lane & 3);           // of four dims
+  const int h = hg / groups, f = (hg - h * groups) * 8 + row;
   const bool in = h < p.c.kv_heads && f < flat;
   const int bt = f / p.group, gi = f - bt * p.group, b = bt / p.s.tokens, t = bt - b * p.s.tokens;
   Walk walk;
   walk.a_cost = OVERHEAD + p.p_tiles;
   walk.a_units = p.joined ? 0 : walk.a_cost * p.a_tiles * p.c.kv_heads;
-  walk.units = __ldcg(p.plan);
-  walk.ctas = (int)__ldcg(p.plan + 1);
+  walk.cut(__ldcg(p.plan), __ldcg(p.plan + 1));
   // parts a0 .. a0 + na - 1 of the prefix, b0 .. b0 + nb - 1 of the sequence's own item
   int a0 = 0, na = 0, b0 = 0, nb = 0, b_row = 0;
   bool done = false;                        // one CTA had it all
   if (in) {
     if (!p.joined && p.p_tiles) {
       const int item = h * p.a_tiles + f / ROWS;
-      const long long u = item * walk.a_cost + OVERHEAD;
+      const int u = item * walk.a_cost + OVERHEAD;
       const int c0 = walk.cta_of(u);
       na = walk.cta_of(u + p.p_tiles - 1) - c0 + 1;
       a0 = c0 + item;
     }
-    const long long s0 = __ldcg(p.plan + 2 + b), s1 = __ldcg(p.plan + 3 + b);
+    const int s0 = __ldcg(p.plan + 2 + b), s1 = __ldcg(p.plan + 3 + b);
     if (s1 > s0) {
       const int fs = f - b * p.s.tokens * p.group, r = fs / p.b_rows, item = (h * p.s.batch + b) * p.b_tiles + r;
       b_row = fs - r * p.b_rows;
-      const long long cost = (s1 - s0) / p.b_tiles, u = walk.a_units + h * __ldcg(p.plan + 2 + p.s.batch) + s0 + r * cost + OVERHEAD;
+      const int cost = (s1 - s0) / p.b_tiles, u = walk.a_units + h * __ldcg(p.plan + 2 + p.s.batch) + s0 + r * cost + OVERHEAD;
       const int c0 = walk.cta_of(u);
       nb = walk.cta_of(u + cost - OVERHEAD - 1) - c0 + 1;
       b0 = c0 + item;
