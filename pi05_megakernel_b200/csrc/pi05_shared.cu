@@ -41,7 +41,7 @@ Cut cut_rows(int sms, const pi05_cache& c, int q_heads, long long batch, long lo
   k.b_tiles = (rows + shared::ROWS - 1) / shared::ROWS;
   k.b_rows = (rows + k.b_tiles - 1) / k.b_tiles;
   k.b_slot = (k.b_rows + 3) / 4 * 4;
-  k.plan_bytes = up256((batch + 3) * 4);
+  k.plan_bytes = up256((k.a_tiles + batch * k.b_tiles) * c.kv_heads * 8);
   k.a_bytes = up256((sms + k.a_tiles * c.kv_heads) * shared::ROWS * (c.head_dim + 2) * 4);
   k.b_bytes = up256((sms + k.b_tiles * batch * c.kv_heads) * k.b_slot * (c.head_dim + 2) * 4);
   return k;
@@ -99,7 +99,7 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   a.grid = (int)std::min<long long>(sms, most);
   a.c_log2 = s.scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.plan = reinterpret_cast<int*>(ws);
+  a.parts = reinterpret_cast<int2*>(ws);
   a.a_parts = reinterpret_cast<float*>(ws + k.plan_bytes);
   a.b_parts = reinterpret_cast<float*>(ws + k.plan_bytes + k.a_bytes);
   a.limit = 2000000000u;                        // about a second
@@ -118,11 +118,13 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   });
   cudaStream_t stream = (cudaStream_t)stream_;
   if (e == cudaSuccess) e = pi05::launch_kernel(attention, a.grid, shared::threads(c.format), smem, stream, 1, true, a);
-  // A row's parts are added by one warp, or by up to eight of a block where there are many: the CTAs' runs over the items they are shared by
-  const long long items = c.kv_heads * (a.joined ? s.batch * k.b_tiles : k.a_tiles), parts = a.grid / items + 1;
-  const int split = parts >= 16 ? 8 : parts >= 8 ? 4 : parts >= 4 ? 2 : 1;
+  // A row's parts are added by one warp, or by up to sixteen of a block where there are many: as many as leave each no more than it loads at once
+  const long long items = c.kv_heads * (a.joined ? s.batch * k.b_tiles : k.a_tiles), parts = a.grid / items + 2;
+  int split = 1;
+  while (split < shared::COMBINE_THREADS / 32 && parts > split * shared::AT_ONCE) split *= 2;
   const long long work = (long long)c.kv_heads * (((long long)s.batch * s.tokens * a.group + 7) / 8) * (c.head_dim / 16);
-  if (e == cudaSuccess) e = pi05::launch_kernel(combine, dim3((unsigned)((work * split + 7) / 8)), 256, 0, stream, 1, true, a, split);
+  const int per = shared::COMBINE_THREADS / 32 / split;
+  if (e == cudaSuccess) e = pi05::launch_kernel(combine, dim3((unsigned)((work + per - 1) / per)), shared::COMBINE_THREADS, 0, stream, 1, true, a, split);
   if (e != cudaSuccess) { cudaGetLastError(); return PI05_ERR_CUDA; }
   return PI05_OK;
 }

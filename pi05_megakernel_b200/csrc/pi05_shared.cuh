@@ -60,7 +60,7 @@ struct Args {
   int p_tiles;                              // tiles of the prefix
   int grid;
   float c_log2;                             // scale x log2 e
-  int* plan;                                // what the combine kernel has to know: {units, CTAs, prefix sums of the sequences' units}
+  int2* parts;                              // of every item, the batch's before the sequences': its first slot, and how many there are (0 or 1 that was finished: none to add)
   float *a_parts, *b_parts;                 // slots of unfinished items: [D / 4][rows][4], then (reference, weight) per row
   uint32_t limit;                           // of a wait, in cycles
 };
@@ -342,9 +342,30 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   ptx::grid_dep_launch();
   const uint32_t tmem = s_tmem;
   const Walk& walk = s_walk;
-  if (blockIdx.x == 0) {
-    for (int b = tid; b <= p.s.batch; b += blockDim.x) p.plan[2 + b] = sums[b];
-    if (tid == 0) { p.plan[0] = walk.units; p.plan[1] = walk.ctas; }
+  // What the combine kernel has to know of the items: the slots of their parts
+  {
+    const int a_items = p.joined ? 0 : p.a_tiles * p.c.kv_heads, items = a_items + p.s.batch * p.c.kv_heads * p.b_tiles;
+    for (int item = tid * gridDim.x + blockIdx.x; item < items; item += gridDim.x * blockDim.x) {
+      int at = 0, tiles = 0;                // first unit behind the item's overhead
+      const int own = item - a_items;
+      if (own < 0) {
+        at = item * walk.a_cost;
+        tiles = p.p_tiles;
+      } else {
+        const int hb = own / p.b_tiles, h = hb / p.s.batch, b = hb - h * p.s.batch, units = sums[b + 1] - sums[b];
+        if (units) {
+          const int cost = units / p.b_tiles;
+          at = walk.a_units + h * walk.b_units + sums[b] + (own - hb * p.b_tiles) * cost;
+          tiles = cost - OVERHEAD;
+        }
+      }
+      int2 part = make_int2(0, 0);
+      if (tiles) {
+        const int first = walk.cta_of(at + OVERHEAD), n = walk.cta_of(at + OVERHEAD + tiles - 1) - first + 1;
+        part = make_int2(first + (own < 0 ? item : own), own >= 0 && p.joined && n == 1 ? -1 : n);
+      }
+      p.parts[item] = part;
+    }
   }
   // Where the keys and values of a segment's tile i of n stand among the segment's units, which is the order of their use: LOOK = 1: K0, K1, V0,
   // K2, V1, .., V(n-1); 2: K0, K1, K2, V0, K3, V1, .., V(n-2), V(n-1).  And what unit u is.
@@ -854,71 +875,78 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   }
 }
 
-// The unfinished items of a launch put together: a warp has eight query rows x 16 dims, of which `split` warps of a block take every split-th
-// part each.
+// The unfinished items of a launch put together.  A warp has eight query rows x 16 dims (a line of every 16 bytes of a part), of which `split` warps of a
+// block take every split-th part each, eight at a time: what bounds it is how many loads are on their way.
+constexpr int COMBINE_THREADS = 512, AT_ONCE = 8;
 template <int DIM>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Args p, int split) {
-  __shared__ float s_m[8][8], s_l[8][8];
-  __shared__ float4 s_o[8][32];
-  ptx::grid_dep_wait();
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const __grid_constant__ Args p, int split) {
+  constexpr int WARPS = COMBINE_THREADS / 32;
+  __shared__ float2 s_ml[WARPS][8];
+  __shared__ float4 s_o[WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, share = warp % split;
   const int flat = p.s.batch * p.s.tokens * p.group, groups = (flat + 7) / 8;
-  const int work = blockIdx.x * (8 / split) + warp / split, hg = work / (DIM / 16);
+  const int work = blockIdx.x * (WARPS / split) + warp / split, hg = work / (DIM / 16);
   const int column = (work & (DIM / 16 - 1)) * 4 + (lane & 3);           // of four dims
   const int h = hg / groups, f = (hg - h * groups) * 8 + row;
   const bool in = h < p.c.kv_heads && f < flat;
   const int bt = f / p.group, gi = f - bt * p.group, b = bt / p.s.tokens, t = bt - b * p.s.tokens;
-  Walk walk;
-  walk.a_cost = OVERHEAD + p.p_tiles;
-  walk.a_units = p.joined ? 0 : walk.a_cost * p.a_tiles * p.c.kv_heads;
-  walk.cut(__ldcg(p.plan), __ldcg(p.plan + 1));
-  // parts a0 .. a0 + na - 1 of the prefix, b0 .. b0 + nb - 1 of the sequence's own item
-  int a0 = 0, na = 0, b0 = 0, nb = 0, b_row = 0;
-  bool done = false;                        // one CTA had it all
+  const int fs = f - b * p.s.tokens * p.group, r = fs / p.b_rows, b_row = fs - r * p.b_rows, a_items = p.joined ? 0 : p.a_tiles * p.c.kv_heads;
+  ptx::grid_dep_wait();
+  int2 a = make_int2(0, 0), o_ = make_int2(0, 0);
   if (in) {
-    if (!p.joined && p.p_tiles) {
-      const int item = h * p.a_tiles + f / ROWS;
-      const int u = item * walk.a_cost + OVERHEAD;
-      const int c0 = walk.cta_of(u);
-      na = walk.cta_of(u + p.p_tiles - 1) - c0 + 1;
-      a0 = c0 + item;
-    }
-    const int s0 = __ldcg(p.plan + 2 + b), s1 = __ldcg(p.plan + 3 + b);
-    if (s1 > s0) {
-      const int fs = f - b * p.s.tokens * p.group, r = fs / p.b_rows, item = (h * p.s.batch + b) * p.b_tiles + r;
-      b_row = fs - r * p.b_rows;
-      const int cost = (s1 - s0) / p.b_tiles, u = walk.a_units + h * __ldcg(p.plan + 2 + p.s.batch) + s0 + r * cost + OVERHEAD;
-      const int c0 = walk.cta_of(u);
-      nb = walk.cta_of(u + cost - OVERHEAD - 1) - c0 + 1;
-      b0 = c0 + item;
-      done = p.joined && nb == 1;
-    }
+    if (!p.joined) a = __ldcg(p.parts + h * p.a_tiles + f / ROWS);
+    o_ = __ldcg(p.parts + a_items + (h * p.s.batch + b) * p.b_tiles + r);
   }
+  const bool done = o_.y < 0;               // one CTA had it all
+  const int n = done ? 0 : a.y + o_.y;
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, float4 v) {
-    const float top = fmaxf(m, ml.x), w0 = m == top ? 1.f : ptx::ex2_approx(m - top), w1 = ml.x == top ? 1.f : ptx::ex2_approx(ml.x - top);
-    l = l * w0 + ml.y * w1;
-    o.x = o.x * w0 + v.x * w1; o.y = o.y * w0 + v.y * w1; o.z = o.z * w0 + v.z * w1; o.w = o.w * w0 + v.w * w1;
+#pragma unroll 1
+  for (int k0 = share; k0 < n; k0 += AT_ONCE * split) {
+    float2 ml[AT_ONCE];
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int at = k0 + k * split;
+      const bool own = at >= a.y;
+      const int rows = own ? p.b_slot : ROWS;
+      const float* part = own ? p.b_parts + (long long)(o_.x + at - a.y) * rows * (DIM + 2) : p.a_parts + (long long)(a.x + at) * rows * (DIM + 2);
+      const int pr = own ? b_row : f % ROWS;
+      ml[k] = at < n ? __ldcg(reinterpret_cast<const float2*>(part + DIM * rows) + pr) : make_float2(-INFINITY, 0.f);
+      v[k] = at < n ? __ldcg(reinterpret_cast<const float4*>(part) + column * rows + pr) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
+    const float w = m == top ? 1.f : ptx::ex2_approx(m - top);
+    l *= w; o.x *= w; o.y *= w; o.z *= w; o.w *= w;
     m = top;
-  };
-  if (!done) {
-#pragma unroll 4
-    for (int k = share; k < na + nb; k += split) {
-      const bool own = k >= na;
-      const int rows = own ? p.b_slot : ROWS, r = own ? b_row : f % ROWS;
-      const float* part = (own ? p.b_parts : p.a_parts) + (long long)(own ? b0 + k - na : a0 + k) * rows * (DIM + 2);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + column * rows + r);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + DIM * rows) + r);
-      add(ml, v);
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const float u = ml[k].x == top ? 1.f : ptx::ex2_approx(ml[k].x - top);
+      l += ml[k].y * u;
+      o.x += v[k].x * u; o.y += v[k].y * u; o.z += v[k].z * u; o.w += v[k].w * u;
     }
   }
   if (split > 1) {
-    if ((lane & 3) == 0) { s_m[warp][row] = m; s_l[warp][row] = l; }
+    if ((lane & 3) == 0) s_ml[warp][row] = make_float2(m, l);
     s_o[warp][lane] = o;
     __syncthreads();
     if (share) return;
-    for (int k = 1; k < split; ++k) add(make_float2(s_m[warp + k][row], s_l[warp + k][row]), s_o[warp + k][lane]);
+    float top = m;
+#pragma unroll 1
+    for (int k = 1; k < split; ++k) top = fmaxf(top, s_ml[warp + k][row].x);
+    const float w = m == top ? 1.f : ptx::ex2_approx(m - top);
+    l *= w; o.x *= w; o.y *= w; o.z *= w; o.w *= w;
+    m = top;
+#pragma unroll 1
+    for (int k = 1; k < split; ++k) {
+      const float2 ml = s_ml[warp + k][row];
+      const float4 v = s_o[warp + k][lane];
+      const float u = ml.x == top ? 1.f : ptx::ex2_approx(ml.x - top);
+      l += ml.y * u;
+      o.x += v.x * u; o.y += v.y * u; o.z += v.z * u; o.w += v.w * u;
+    }
   }
   if (!in || done) return;
   const float il = l == 0.f ? 0.f : 1.0f / l;
