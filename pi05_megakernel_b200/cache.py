@@ -9,6 +9,7 @@ current stream; the work is done by ``libpi05_b200.so``.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -16,10 +17,22 @@ from . import _lib
 
 FORMATS = {"bf16": (_lib.CACHE_BF16, torch.bfloat16), "int8": (_lib.CACHE_INT8, torch.int8), "e4m3": (_lib.CACHE_E4M3, torch.float8_e4m3fn)}
 
+ROWS = struct.Struct("@PP4qPPP6i")           # pi05_cache_rows of the header
+MAX_FITS = 256                                # shapes whose checks are kept
+
 
 def check_table(name: str, t: torch.Tensor, device: torch.device, dim: int) -> None:
     if t.dtype != torch.int32 or t.dim() != dim or t.device != device or (t.numel() > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name} must be an int32 tensor of {dim} dimensions on {device}, contiguous along its last")
+
+
+# The current stream of a device as an integer; the public way to it makes an object, which takes 2 us of a call that takes 6.
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def describe(t: torch.Tensor | None):
+    """What a check of a table goes by."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def strides(t: torch.Tensor) -> list[int]:
@@ -75,19 +88,22 @@ class KvCache:
         self.words = torch.zeros(4, dtype=torch.int32, device=self.device)       # the status words
         scale = (None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())
         self.struct = _lib.Cache(k.data_ptr(), v.data_ptr(), *scale, self.words.data_ptr(), FORMATS[self.format][0], *k.shape)
-        self.ref = ctypes.byref(self.struct)
+        self.ref, self.index, self.fits = ctypes.byref(self.struct), self.device.index, {}
+        self.call_write, self.call_read = self.lib.pi05_cache_write, self.lib.pi05_cache_read
         # what the library refuses is refused here, before a first call
         nbytes = ctypes.c_size_t()
         _lib.check(self.lib, None, self.lib.pi05_shared_workspace(1, self.ref, self.kv_heads, 1, 1, ctypes.byref(nbytes)))
 
-    def _rows(self, k, v, table, starts, counts, layer):
+    def _fit(self, k, v, table, starts, counts, layer):
+        """What does not depend on addresses, checked: the strides and sizes of the call.  Kept by shapes and types, since checking costs as much as
+        a small call."""
         if k.dim() != 5 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != self.device or v.device != self.device:
             raise ValueError(f"k and v must be bfloat16 [batch, layers, tokens, kv_heads, head_dim] on {self.device}")
         batch, layers, tokens, heads, dim = k.shape
         if heads != self.kv_heads or dim != self.head_dim or layer < 0 or layer + layers > self.layers:
             raise ValueError(f"{tuple(k.shape)} from layer {layer} on does not fit a cache of {self.layers} layers x {self.kv_heads} heads of {self.head_dim}")
         st = strides(k)
-        if st != strides(v) or k.stride(4) != 1 or v.stride(4) != 1 or any(s % 8 for s in st) or (k.data_ptr() | v.data_ptr()) % 16:
+        if st != strides(v) or k.stride(4) != 1 or v.stride(4) != 1 or any(s % 8 for s in st):
             raise ValueError("k and v must share their strides (multiples of 8 elements, the last dimension contiguous) and be 16-byte aligned")
         check_table("table", table, self.device, 2)
         if table.shape[0] != batch:
@@ -97,9 +113,19 @@ class KvCache:
                 check_table(name, t, self.device, 1)
                 if t.shape[0] != batch:
                     raise ValueError(f"{name} needs an entry per sequence")
-        return _lib.CacheRows(k.data_ptr(), v.data_ptr(), *st, table.data_ptr(), None if starts is None else starts.data_ptr(),
-                              None if counts is None else counts.data_ptr(), batch, layers, tokens, layer, table.stride(0) if batch > 1 else table.shape[1],
-                              table.shape[1])
+        return (*st, batch, layers, tokens, layer, table.stride(0) if batch > 1 else table.shape[1], table.shape[1])
+
+    def _rows(self, k, v, table, starts, counts, layer) -> bytes:
+        key = (k.shape, v.shape, k.stride(), v.stride(), k.dtype, v.dtype, k.device, v.device, layer, describe(table), describe(starts), describe(counts))
+        fit = self.fits.get(key)
+        if fit is None:
+            if len(self.fits) >= MAX_FITS:
+                self.fits.clear()
+            fit = self.fits[key] = self._fit(k, v, table, starts, counts, layer)
+        kp, vp = k.data_ptr(), v.data_ptr()
+        if (kp | vp) & 15:
+            raise ValueError("k and v must share their strides (multiples of 8 elements, the last dimension contiguous) and be 16-byte aligned")
+        return ROWS.pack(kp, vp, *fit[:4], table.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), *fit[4:])
 
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor | None = None,
               counts: torch.Tensor | None = None, layer: int = 0) -> None:
@@ -107,22 +133,24 @@ class KvCache:
         strides that they share go to layers ``layer`` .. of the cache and to the tokens ``starts[b]`` .. (None: 0 ..) of sequence ``b``, whose
         pages ``table`` int32 ``[batch, pages]`` names; of a padded batch only the first ``counts[b]`` tokens are taken.  Tokens of one call must
         lie in different places of the cache."""
-        rows = self._rows(k, v, table, starts, counts, layer)
-        _lib.check(self.lib, None, self.lib.pi05_cache_write(self.device.index, self.ref, ctypes.byref(rows),
-                                                             torch.cuda.current_stream(self.device).cuda_stream))
+        rc = self.call_write(self.index, self.ref, self._rows(k, v, table, starts, counts, layer), raw_stream(self.index))
+        if rc:
+            _lib.check(self.lib, None, rc)
 
     def read(self, table: torch.Tensor, tokens: int, starts: torch.Tensor | None = None, counts: torch.Tensor | None = None, layer: int = 0,
              layers: int | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows out of their pages, asynchronous on the current stream: BF16 keys and values ``[batch, layers, tokens, kv_heads, head_dim]`` of
         layers ``layer`` .. (all that there are), zeros behind ``counts[b]``; the rest as in ``write``."""
+        if layers is None:
+            layers = self.layers - layer
         if out is None:
-            shape = (table.shape[0], self.layers - layer if layers is None else layers, tokens, self.kv_heads, self.head_dim)
+            shape = (table.shape[0], layers, tokens, self.kv_heads, self.head_dim)
             out = (torch.empty(shape, dtype=torch.bfloat16, device=self.device), torch.empty(shape, dtype=torch.bfloat16, device=self.device))
-        elif out[0].shape[1:3] != (self.layers - layer if layers is None else layers, tokens):
+        elif out[0].shape[1:3] != (layers, tokens):
             raise ValueError("out does not have the layers and tokens that are read")
-        rows = self._rows(*out, table, starts, counts, layer)
-        _lib.check(self.lib, None, self.lib.pi05_cache_read(self.device.index, self.ref, ctypes.byref(rows),
-                                                            torch.cuda.current_stream(self.device).cuda_stream))
+        rc = self.call_read(self.index, self.ref, self._rows(*out, table, starts, counts, layer), raw_stream(self.index))
+        if rc:
+            _lib.check(self.lib, None, rc)
         return out
 
     def status(self) -> None:

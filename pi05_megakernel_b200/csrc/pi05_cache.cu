@@ -1,8 +1,9 @@
 // Rows of keys and values into the pages of a cache, and out of them.
 //
-// Both are one pass over their data, bound by memory: a row (head_dim elements of one token, head and layer) is taken by
-// head_dim / 8 neighbouring lanes, 16 bytes of BF16 each, keys and values by the same lanes so that a thread has two rows on
-// their way and looks the page up once.
+// Both are one pass over their data.  A row (head_dim elements of one token, head and layer) is taken by neighbouring lanes, 16 elements of an 8-bit
+// cache each (8 of a BF16 one), keys and values by the same lanes, so that a thread has four loads on their way and looks the page up once.
+// What bounds them is memory as long as a pair of elements costs no more than some 30 instructions: hence 16 elements a lane (the page, the row's
+// maximum and its quotient once for them) and arithmetic in pairs.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -22,22 +23,21 @@ constexpr int BLOCK = 256;
 struct RowArgs {
   pi05_cache c;
   pi05_cache_rows r;
-  long long rows;                 // batch x tokens x heads, of one layer
+  unsigned rows;                  // tokens x heads, of one sequence and layer
 };
 
 // Where a row of the call is: in the caller's tensors and in the pool (element offsets), and its scale.
-struct Place { long long mine; long long pool; long long scale; int sequence; bool has, good; };
+struct Place { long long mine, pool, scale; bool has, good; };
 
-__device__ __forceinline__ Place place(const RowArgs& a, int row, int layer) {
+__device__ __forceinline__ Place place(const RowArgs& a, unsigned row, int layer, int b) {
   const pi05_cache& c = a.c;
   const pi05_cache_rows& r = a.r;
   Place p;
-  const int head = row % c.kv_heads, bt = row / c.kv_heads, t = bt % r.tokens, b = bt / r.tokens;
-  p.sequence = b;
+  const unsigned t = row / (unsigned)c.kv_heads, head = row - t * (unsigned)c.kv_heads;
   p.mine = b * r.batch_stride + layer * r.layer_stride + t * r.token_stride + head * r.head_stride;
-  p.has = !r.counts || t < __ldg(r.counts + b);
+  p.has = !r.counts || (int)t < __ldg(r.counts + b);
   const int start = r.starts ? __ldg(r.starts + b) : 0;
-  const unsigned pos = (unsigned)start + (unsigned)t, lp = pos / (unsigned)c.page_tokens, at = pos - lp * (unsigned)c.page_tokens;
+  const unsigned pos = (unsigned)start + t, lp = pos / (unsigned)c.page_tokens, at = pos - lp * (unsigned)c.page_tokens;
   p.good = start >= 0 && lp < (unsigned)r.table_pages;
   int page = -1;
   if (p.has) {
@@ -58,108 +58,134 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Eight elements of a row as codes, and the row's scale.
+// Sixteen elements of a row as codes, and the row's scale.
 //   code = rn(x * peak / a) of the true quotient, a the row's largest magnitude.  With BF16 x and a the quotient is either in the middle of
 // two codes exactly (x = a / 2 is 63.5) or at least 2^-10 away from it, so it only has to be right to that, and exact in the middle: peak / a as
-// the sum of two FP32 numbers, and x times it as one FMA on top of the small product, which rounds once.
+// the sum of two FP32 numbers (the reciprocal, a step of Newton's and what that leaves), and x times it as one FMA on top of the small product, which
+// rounds once.
 template <int FORMAT, int LANES>
-__device__ __forceinline__ uint2 encode(const uint4& x, float* scale) {
-  constexpr float PEAK = FORMAT == PI05_CACHE_INT8 ? 127.0f : 448.0f;
-  const uint32_t m = 0x7fff7fffu;
-  uint32_t top = max_pair(max_pair(x.x & m, x.y & m), max_pair(x.z & m, x.w & m));
+__device__ __forceinline__ uint4 encode(const uint4 (&x)[2], float* scale) {
+  constexpr float PEAK = FORMAT == PI05_CACHE_INT8 ? 127.0f : 448.0f, ONE_PEAKTH = 1.0f / PEAK;
+  const uint32_t m = 0x7fff7fffu, w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+  uint32_t top = max_pair(max_pair(max_pair(w[0] & m, w[1] & m), max_pair(w[2] & m, w[3] & m)), max_pair(max_pair(w[4] & m, w[5] & m), max_pair(w[6] & m, w[7] & m)));
+  top = max_pair(top, __byte_perm(top, 0, 0x1032));                // both halves
 #pragma unroll
   for (int d = LANES / 2; d; d >>= 1) top = max_pair(top, __shfl_xor_sync(0xffffffffu, top, d));
-  top = max_pair(top, top >> 16);                                  // (the shift brings zeros to the other half)
-  float a = lo16(top);
-  *scale = __fdiv_rn(a, PEAK);
-  float v[8] = {lo16(x.x), hi16(x.x), lo16(x.y), hi16(x.y), lo16(x.z), hi16(x.z), lo16(x.w), hi16(x.w)};
+  float a = lo16(top), f = 1.f;
   if (!(a > 0.f && a <= 3.3895314e38f)) {                          // nothing but zeros; an infinity or a NaN: the whole row reads back as NaN
-    if (a != 0.f) *scale = __uint_as_float(0x7fffffffu);
-    return make_uint2(0u, 0u);
+    *scale = a == 0.f ? 0.f : __uint_as_float(0x7fffffffu);
+    return make_uint4(0u, 0u, 0u, 0u);
   }
-  if (!(a > 1e-30f && a < 1e30f)) {                                // keep peak / a and the products away from the ends of FP32: both times a power of two
-    const float f = a < 1.f ? 0x1p+90f : 0x1p-90f;
+  if (!(a > 1e-30f && a < 1e30f)) {                                // keep quotient and products away from the ends of FP32: both times a power of two
+    f = a < 1.f ? 0x1p+90f : 0x1p-90f;
+    *scale = __fdiv_rn(a, PEAK);
     a *= f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= f;
+  } else {
+    const float q = a * ONE_PEAKTH;
+    *scale = fmaf(fmaf(-q, PEAK, a), ONE_PEAKTH, q);               // a / peak, rounded once
   }
-  const float hi = __fdiv_rn(PEAK, a), lo = __fdiv_rn(fmaf(-hi, a, PEAK), a);
-  uint32_t w[2];
+  const float r = ptx::rcp_approx(a), h = PEAK * r, hi = fmaf(fmaf(-h, a, PEAK), r, h), lo = fmaf(-hi, a, PEAK) * r;
+  const float2 hi2 = make_float2(hi, hi), lo2 = make_float2(lo, lo), zero = make_float2(0.f, 0.f), f2 = make_float2(f, f);
+  uint32_t code[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float y[4];
+  for (int k = 0; k < 4; ++k) {
+    float2 y[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = fmaf(v[4 * h + i], hi, v[4 * h + i] * lo);
+    for (int i = 0; i < 2; ++i) {
+      float2 v = make_float2(lo16(w[2 * k + i]), hi16(w[2 * k + i]));
+      if (f != 1.f) { v.x *= f2.x; v.y *= f2.y; }
+      y[i] = ptx::fma2(v, hi2, ptx::fma2(v, lo2, zero));
+    }
     if (FORMAT == PI05_CACHE_INT8) {
       // to the nearest whole number, ties to even, by a sum whose last place is 1; its last byte is the code
-      uint32_t n[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) n[i] = __float_as_uint(y[i] + 12582912.0f);
-      w[h] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+      const uint32_t a0 = __float_as_uint(y[0].x + 12582912.0f), a1 = __float_as_uint(y[0].y + 12582912.0f), a2 = __float_as_uint(y[1].x + 12582912.0f),
+                     a3 = __float_as_uint(y[1].y + 12582912.0f);
+      code[k] = __byte_perm(__byte_perm(a0, a1, 0x0040), __byte_perm(a2, a3, 0x0040), 0x5410);
     } else {
       unsigned short p[2];
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[0]) : "f"(y[1]), "f"(y[0]));
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[1]) : "f"(y[3]), "f"(y[2]));
-      w[h] = p[0] | (uint32_t)p[1] << 16;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[0]) : "f"(y[0].y), "f"(y[0].x));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p[1]) : "f"(y[1].y), "f"(y[1].x));
+      code[k] = p[0] | (uint32_t)p[1] << 16;
     }
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint4(code[0], code[1], code[2], code[3]);
 }
+
+__host__ __device__ constexpr int lanes(int format, int dim) { return dim / (format == PI05_CACHE_BF16 ? 8 : 16); }
 
 template <int FORMAT, int DIM>
 __global__ void __launch_bounds__(BLOCK) write_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int LANES = DIM / 8;
-  const int lane = threadIdx.x % LANES, layer = blockIdx.y;
-  const long long row = (long long)blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = lanes(FORMAT, DIM);
+  const int lane = threadIdx.x % LANES;
+  const unsigned row = blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
   const bool in = row < a.rows;                                    // (every lane takes part in the shuffles)
-  const Place p = place(a, in ? (int)row : 0, layer);
+  const Place p = place(a, in ? row : 0, blockIdx.y, blockIdx.z);
   const bool store = in && p.has && p.good;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const __nv_bfloat16 *sk = static_cast<const __nv_bfloat16*>(a.r.k) + p.mine, *sv = static_cast<const __nv_bfloat16*>(a.r.v) + p.mine;
-  const uint4 k = store ? __ldcs(reinterpret_cast<const uint4*>(sk) + lane) : zero, v = store ? __ldcs(reinterpret_cast<const uint4*>(sv) + lane) : zero;
+  const uint4* sk = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.k) + p.mine);
+  const uint4* sv = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.v) + p.mine);
   if constexpr (FORMAT == PI05_CACHE_BF16) {
     if (!store) return;
+    const uint4 k = __ldcs(sk + lane), v = __ldcs(sv + lane);
     reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.k) + p.pool)[lane] = k;
     reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.v) + p.pool)[lane] = v;
   } else {
+    uint4 k[2], v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      k[i] = store ? __ldcs(sk + 2 * lane + i) : zero;
+      v[i] = store ? __ldcs(sv + 2 * lane + i) : zero;
+    }
     float ks, vs;
-    const uint2 kc = encode<FORMAT, LANES>(k, &ks), vc = encode<FORMAT, LANES>(v, &vs);
+    const uint4 kc = encode<FORMAT, LANES>(k, &ks), vc = encode<FORMAT, LANES>(v, &vs);
     if (!store) return;
-    reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.c.k) + p.pool)[lane] = kc;
-    reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.c.v) + p.pool)[lane] = vc;
+    reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.c.k) + p.pool)[lane] = kc;
+    reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.c.v) + p.pool)[lane] = vc;
     if (lane == 0) { a.c.k_scale[p.scale] = ks; a.c.v_scale[p.scale] = vs; }
   }
 }
 
+// Eight of a lane's codes as BF16 values: the code as a 16-bit number, exactly, times the scale in FP32.
 template <int FORMAT>
-__device__ __forceinline__ uint4 decode(const void* pool, long long at, int lane, float scale) {
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at) + lane);
-  const uint2 a = cache::quad<FORMAT>(w.x), b = cache::quad<FORMAT>(w.y);
+__device__ __forceinline__ uint4 decode(uint32_t lo, uint32_t hi, float scale) {
+  const uint2 a = cache::quad<FORMAT>(lo), b = cache::quad<FORMAT>(hi);
   return make_uint4(pack2(lo16(a.x) * scale, hi16(a.x) * scale), pack2(lo16(a.y) * scale, hi16(a.y) * scale),
                     pack2(lo16(b.x) * scale, hi16(b.x) * scale), pack2(lo16(b.y) * scale, hi16(b.y) * scale));
 }
 
 template <int FORMAT, int DIM>
 __global__ void __launch_bounds__(BLOCK) read_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int LANES = DIM / 8;
-  const int lane = threadIdx.x % LANES, layer = blockIdx.y;
-  const long long row = (long long)blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = lanes(FORMAT, DIM);
+  const int lane = threadIdx.x % LANES;
+  const unsigned row = blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
   if (row >= a.rows) return;
-  const Place p = place(a, (int)row, layer);
-  uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
-  if (p.has && p.good) {
-    if constexpr (FORMAT == PI05_CACHE_BF16) {
-      k = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.k) + p.pool) + lane);
-      v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.v) + p.pool) + lane);
-    } else {
-      k = decode<FORMAT>(a.c.k, p.pool, lane, __ldg(a.c.k_scale + p.scale));
-      v = decode<FORMAT>(a.c.v, p.pool, lane, __ldg(a.c.v_scale + p.scale));
+  const Place p = place(a, row, blockIdx.y, blockIdx.z);
+  uint4* dk = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.k) + p.mine);
+  uint4* dv = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.v) + p.mine);
+  // behind the sequence's tokens zeros; where there is no such page NaN, so that nobody takes it for a key
+  const uint32_t none = p.has ? 0x7fff7fffu : 0u;
+  uint4 k[2] = {make_uint4(none, none, none, none), make_uint4(none, none, none, none)}, v[2] = {k[0], k[0]};
+  if constexpr (FORMAT == PI05_CACHE_BF16) {
+    if (p.has && p.good) {
+      k[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.k) + p.pool) + lane);
+      v[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.v) + p.pool) + lane);
     }
-  } else if (p.has) {
-    k = v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);      // no such page: NaN, so that nobody takes it for a key
+    __stcs(dk + lane, k[0]);
+    __stcs(dv + lane, v[0]);
+  } else {
+    if (p.has && p.good) {
+      const uint4 kc = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.c.k) + p.pool) + lane);
+      const uint4 vc = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.c.v) + p.pool) + lane);
+      const float ks = __ldg(a.c.k_scale + p.scale), vs = __ldg(a.c.v_scale + p.scale);
+      k[0] = decode<FORMAT>(kc.x, kc.y, ks); k[1] = decode<FORMAT>(kc.z, kc.w, ks);
+      v[0] = decode<FORMAT>(vc.x, vc.y, vs); v[1] = decode<FORMAT>(vc.z, vc.w, vs);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      __stcs(dk + 2 * lane + i, k[i]);
+      __stcs(dv + 2 * lane + i, v[i]);
+    }
   }
-  __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.k) + p.mine) + lane, k);
-  __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.v) + p.mine) + lane, v);
 }
 
 typedef void (*RowKernel)(const RowArgs);
@@ -180,17 +206,17 @@ int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c,
   if (r->batch < 0 || r->tokens < 0 || r->layers < 0 || r->layer < 0 || r->layer > c->layers - r->layers || r->table_pages < 0 || r->table_stride < 0)
     return PI05_ERR_ARGUMENT;
   if (r->batch == 0 || r->tokens == 0 || r->layers == 0) return PI05_OK;
-  const long long rows = (long long)r->batch * r->tokens * c->kv_heads;
-  if (!r->k || !r->v || !r->table || rows > 0x7fffffffll || (long long)r->batch * r->tokens > 0x7fffffffll) return PI05_ERR_ARGUMENT;
+  const long long rows = (long long)r->tokens * c->kv_heads;
+  if (!r->k || !r->v || !r->table || rows > 0x7fffffffll || r->batch > 65535 || r->layers > 65535) return PI05_ERR_ARGUMENT;
   if ((((uintptr_t)r->k | (uintptr_t)r->v) & 15) || ((r->batch_stride | r->layer_stride | r->token_stride | r->head_stride) & 7) ||
       (((uintptr_t)r->table | (uintptr_t)r->starts | (uintptr_t)r->counts) & 3))
     return PI05_ERR_ARGUMENT;
   DeviceGuard guard(device);
   if (!guard.ok) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
-  const int per = BLOCK / (c->head_dim / 8);
-  const RowArgs a = {*c, *r, rows};
+  const int per = BLOCK / lanes(c->format, c->head_dim);
+  const RowArgs a = {*c, *r, (unsigned)rows};
   const RowKernel kernel = kernels[c->format][c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2];
-  kernel<<<dim3((unsigned)((rows + per - 1) / per), r->layers), BLOCK, 0, (cudaStream_t)stream>>>(a);
+  kernel<<<dim3((unsigned)((rows + per - 1) / per), r->layers, r->batch), BLOCK, 0, (cudaStream_t)stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? PI05_OK : PI05_ERR_CUDA;
 }
 

@@ -9,11 +9,14 @@ one pass, or the tokens of several action chunks.  torch only supplies device me
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _lib
-from .cache import KvCache, check_table, strides
+from .cache import MAX_FITS, KvCache, check_table, describe, raw_stream, strides
+
+CALL = struct.Struct("@PPP6qPPPP8if4x")      # pi05_shared_call of the header
 
 
 class SharedPrefixAttention:
@@ -29,6 +32,7 @@ class SharedPrefixAttention:
         sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         _lib.check(self.lib, None, self.lib.pi05_shared_workspace(sms, cache.ref, q_heads, max_batch, max_tokens, ctypes.byref(nbytes)))
         self.ws = torch.zeros(nbytes.value, dtype=torch.uint8, device=self.device)
+        self.workspace, self.nbytes, self.index, self.fits, self.call = self.ws.data_ptr(), nbytes.value, self.device.index, {}, self.lib.pi05_shared_attention
 
     def run(self, q: torch.Tensor, prefix_table: torch.Tensor | None, prefix_tokens: int, table: torch.Tensor | None = None,
             lengths: torch.Tensor | None = None, layer: int = 0, valid: torch.Tensor | None = None, causal: bool = True,
@@ -40,6 +44,29 @@ class SharedPrefixAttention:
         of them count (None: all).  ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` are the sequences' own tokens, the
         queries' among them; ``causal``: query t sees own tokens up to its own place, ``lengths[b] - tokens + t``, else all of them.
         ``scale`` defaults to head_dim ** -0.5.  A query that sees no key gets zeros (log-sum-exp: -infinity)."""
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        key = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device, describe(prefix_table), prefix_tokens, describe(table),
+               describe(lengths), describe(valid), layer, causal, scale)
+        fit = self.fits.get(key)
+        if fit is None:
+            if len(self.fits) >= MAX_FITS:
+                self.fits.clear()
+            fit = self.fits[key] = self._fit(q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale)
+        qp, op = q.data_ptr(), out.data_ptr()
+        if (qp | op) & 15:
+            raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=self.device) if with_lse else None
+        call = CALL.pack(qp, op, lse.data_ptr() if with_lse else 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0,
+                         valid.data_ptr() if prefix_tokens and valid is not None else 0, 0 if table is None else table.data_ptr(),
+                         0 if lengths is None else lengths.data_ptr(), *fit[6:])
+        rc = self.call(self.index, self.cache.ref, call, self.workspace, self.nbytes, raw_stream(self.index))
+        if rc:
+            _lib.check(self.lib, None, rc)
+        return (out, lse) if with_lse else out
+
+    def _fit(self, q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale):
+        """What does not depend on addresses, checked, as in ``KvCache``."""
         c = self.cache
         if q.dim() != 4 or q.dtype != torch.bfloat16 or q.device != self.device or q.shape[2] != self.q_heads or q.shape[3] != c.head_dim:
             raise ValueError(f"q must be bfloat16 [batch, tokens, {self.q_heads}, {c.head_dim}] on {self.device}")
@@ -49,12 +76,10 @@ class SharedPrefixAttention:
         scale = c.head_dim ** -0.5 if scale is None else scale
         if not 0 <= layer < c.layers or prefix_tokens < 0 or not 0 < scale < float("inf"):
             raise ValueError("no such layer in the cache, a negative prefix_tokens, or a scale that is not positive and finite")
-        if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-        elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device:
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device:
             raise ValueError("out must be like q")
         qs, os_ = strides(q), strides(out)
-        if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_) or (q.data_ptr() | out.data_ptr()) % 16:
+        if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_):
             raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
         if prefix_tokens:
             if prefix_table is None:
@@ -66,20 +91,14 @@ class SharedPrefixAttention:
                 raise ValueError(f"valid must be a contiguous bool tensor [{prefix_tokens}] on {self.device}")
         if (table is None) != (lengths is None):
             raise ValueError("own tokens need a table and lengths")
+        pages = 0
         if table is not None:
             check_table("table", table, self.device, 2)
             check_table("lengths", lengths, self.device, 1)
             if table.shape[0] != batch or lengths.shape[0] != batch:
                 raise ValueError("table and lengths need an entry per sequence")
-        lse = torch.empty((batch, tokens, self.q_heads), dtype=torch.float32, device=self.device) if with_lse else None
-        ptr = lambda t: None if t is None else t.data_ptr()
-        call = _lib.SharedCall(q.data_ptr(), out.data_ptr(), ptr(lse), *qs, *os_, ptr(prefix_table) if prefix_tokens else None,
-                               ptr(valid) if prefix_tokens else None, ptr(table), ptr(lengths), batch, tokens, self.q_heads, layer, prefix_tokens,
-                               0 if table is None else table.stride(0) if batch > 1 else table.shape[1], 0 if table is None else table.shape[1],
-                               bool(causal), scale)
-        _lib.check(self.lib, None, self.lib.pi05_shared_attention(self.device.index, c.ref, ctypes.byref(call), self.ws.data_ptr(), self.ws.numel(),
-                                                                  torch.cuda.current_stream(self.device).cuda_stream))
-        return (out, lse) if with_lse else out
+            pages = table.shape[1]
+        return (*qs, *os_, batch, tokens, self.q_heads, layer, prefix_tokens, table.stride(0) if pages and batch > 1 else pages, pages, bool(causal), scale)
 
     def status(self) -> None:
         """``KvCache.status`` of the cache."""

@@ -23,14 +23,14 @@ def cache(**change):
 def rows(**change):
     fields = dict(k=0x60000, v=0x70000, batch_stride=4096, layer_stride=2048, token_stride=256, head_stride=128, table=0x80000, starts=None,
                   counts=None, batch=2, layers=2, tokens=8, layer=0, table_stride=4, table_pages=4)
-    return _lib.CacheRows(**{**fields, **change})
+    return ctypes.byref(_lib.CacheRows(**{**fields, **change}))
 
 
 def call(**change):
     fields = dict(q=0x60000, out=0x70000, lse=None, q_batch_stride=1024, q_token_stride=1024, q_head_stride=128, out_batch_stride=1024,
                   out_token_stride=1024, out_head_stride=128, prefix_table=0x80000, prefix_valid=None, table=0x90000, lengths=0xa0000, batch=2, tokens=1,
                   q_heads=8, layer=0, prefix_tokens=100, table_stride=4, table_pages=4, causal=1, scale=1.0)
-    return _lib.SharedCall(**{**fields, **change})
+    return ctypes.byref(_lib.SharedCall(**{**fields, **change}))
 
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(status=None), dict(k=0x10008), dict(v_scale=0x40004), dict(k_scale=None), dict(format=3), dict(format=-1),
@@ -50,7 +50,7 @@ def test_bad_caches_are_refused(lib, change):
 
 BAD_ROWS = [dict(k=None), dict(v=None), dict(table=None), dict(k=0x60008), dict(batch=-1), dict(tokens=-1), dict(layers=-1), dict(layers=3), dict(layer=1),
             dict(layer=-1), dict(token_stride=260), dict(head_stride=4), dict(batch_stride=2), dict(table=0x80002), dict(table_pages=-1),
-            dict(table_stride=-1), dict(counts=0x1), dict(starts=0x2), dict(batch=1 << 16, tokens=1 << 16)]
+            dict(table_stride=-1), dict(counts=0x1), dict(starts=0x2), dict(batch=1 << 16), dict(tokens=1 << 30)]
 
 
 @pytest.mark.parametrize("change", BAD_ROWS, ids=[str(c) for c in BAD_ROWS])
@@ -115,6 +115,18 @@ def test_python_refuses_a_bad_cache(change):
     from pi05_megakernel_b200.cache import KvCache
     with pytest.raises(ValueError):
         KvCache(**{**dict(pages=4, layers=1, page_tokens=64, kv_heads=1, head_dim=256, format="int8"), **change})
+
+
+def test_packed_arguments_are_the_structures():
+    """The Python classes pack the structures of the header by themselves: same sizes and places."""
+    from pi05_megakernel_b200 import cache as C
+    from pi05_megakernel_b200 import shared as S
+    for packed, fields in ((C.ROWS, _lib.CacheRows), (S.CALL, _lib.SharedCall)):
+        assert packed.size == ctypes.sizeof(fields)
+        values = [i + 1 for i in range(len(fields._fields_))]
+        raw = packed.pack(*values)
+        got = fields.from_buffer_copy(raw)
+        assert [getattr(got, name) for name, _ in fields._fields_] == values
 
 
 def test_error_string_of_a_page_table(lib):
