@@ -1,9 +1,8 @@
 // Rows of keys and values into the pages of a cache, and out of them.
 //
-// Both are one pass over their data.  A row (head_dim elements of one token, head and layer) is taken by neighbouring lanes, 16 elements of an 8-bit
-// cache each (8 of a BF16 one), keys and values by the same lanes, so that a thread has four loads on their way and looks the page up once.
-// What bounds them is memory as long as a pair of elements costs no more than some 30 instructions: hence 16 elements a lane (the page, the row's
-// maximum and its quotient once for them) and arithmetic in pairs.
+// Both are one pass over their data.  A row (head_dim elements of one token, head and layer) is taken by neighbouring lanes, 16 elements each, keys and
+// values by the same lanes, which look the page up once.  What bounds them is memory as long as a pair of elements costs no more than some 30
+// instructions: hence 16 elements a lane (the page, the row's maximum and its quotient once for them) and arithmetic in pairs.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -18,12 +17,13 @@ using cache::hi16;
 using cache::lo16;
 using cache::pack2;
 
-constexpr int BLOCK = 256;
+constexpr int BLOCK = 128;
 
 struct RowArgs {
   pi05_cache c;
   pi05_cache_rows r;
   unsigned rows;                  // tokens x heads, of one sequence and layer
+  int wide;                       // rows of 16-bit elements begin on 32 bytes
 };
 
 // Where a row of the call is: in the caller's tensors and in the pool (element offsets), and its scale.
@@ -49,6 +49,27 @@ __device__ __forceinline__ Place place(const RowArgs& a, unsigned row, int layer
   p.pool = ((pl * c.page_tokens + at) * c.kv_heads + head) * c.head_dim;
   p.scale = (pl * c.kv_heads + head) * c.page_tokens + at;
   return p;
+}
+
+// A lane's 32 bytes, in one piece where they are aligned (two pieces of 16 leave the gaps of a warp's line to the other one: sixteen prefixes of 968 tokens
+// are read back in 60 us in one piece, in 78 in two).
+__device__ __forceinline__ void load_32(uint4 (&x)[2], const uint4* from, bool wide) {
+  if (wide) {
+    asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(x[0].x), "=r"(x[0].y), "=r"(x[0].z), "=r"(x[0].w), "=r"(x[1].x), "=r"(x[1].y), "=r"(x[1].z), "=r"(x[1].w) : "l"(from));
+  } else {
+    x[0] = __ldcs(from);
+    x[1] = __ldcs(from + 1);
+  }
+}
+__device__ __forceinline__ void store_32(uint4* to, const uint4 (&x)[2], bool wide) {
+  if (wide) {
+    asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(to), "r"(x[0].x), "r"(x[0].y), "r"(x[0].z), "r"(x[0].w), "r"(x[1].x), "r"(x[1].y), "r"(x[1].z), "r"(x[1].w) : "memory");
+  } else {
+    __stcs(to, x[0]);
+    __stcs(to + 1, x[1]);
+  }
 }
 
 // Largest magnitude of a pair of BF16, NaN where there is one.
@@ -111,31 +132,24 @@ __device__ __forceinline__ uint4 encode(const uint4 (&x)[2], float* scale) {
   return make_uint4(code[0], code[1], code[2], code[3]);
 }
 
-__host__ __device__ constexpr int lanes(int format, int dim) { return dim / (format == PI05_CACHE_BF16 ? 8 : 16); }
-
 template <int FORMAT, int DIM>
 __global__ void __launch_bounds__(BLOCK) write_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int LANES = lanes(FORMAT, DIM);
+  constexpr int LANES = DIM / 16;
   const int lane = threadIdx.x % LANES;
   const unsigned row = blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
   const bool in = row < a.rows;                                    // (every lane takes part in the shuffles)
   const Place p = place(a, in ? row : 0, blockIdx.y, blockIdx.z);
   const bool store = in && p.has && p.good;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const uint4* sk = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.k) + p.mine);
-  const uint4* sv = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.v) + p.mine);
+  uint4 k[2] = {}, v[2] = {};
+  if (store) {
+    load_32(k, reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.k) + p.mine) + 2 * lane, a.wide);
+    load_32(v, reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.r.v) + p.mine) + 2 * lane, a.wide);
+  }
   if constexpr (FORMAT == PI05_CACHE_BF16) {
     if (!store) return;
-    const uint4 k = __ldcs(sk + lane), v = __ldcs(sv + lane);
-    reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.k) + p.pool)[lane] = k;
-    reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.v) + p.pool)[lane] = v;
+    store_32(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.k) + p.pool) + 2 * lane, k, a.wide);
+    store_32(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.v) + p.pool) + 2 * lane, v, a.wide);
   } else {
-    uint4 k[2], v[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      k[i] = store ? __ldcs(sk + 2 * lane + i) : zero;
-      v[i] = store ? __ldcs(sv + 2 * lane + i) : zero;
-    }
     float ks, vs;
     const uint4 kc = encode<FORMAT, LANES>(k, &ks), vc = encode<FORMAT, LANES>(v, &vs);
     if (!store) return;
@@ -155,37 +169,28 @@ __device__ __forceinline__ uint4 decode(uint32_t lo, uint32_t hi, float scale) {
 
 template <int FORMAT, int DIM>
 __global__ void __launch_bounds__(BLOCK) read_kernel(const __grid_constant__ RowArgs a) {
-  constexpr int LANES = lanes(FORMAT, DIM);
+  constexpr int LANES = DIM / 16;
   const int lane = threadIdx.x % LANES;
   const unsigned row = blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES;
   if (row >= a.rows) return;
   const Place p = place(a, row, blockIdx.y, blockIdx.z);
-  uint4* dk = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.k) + p.mine);
-  uint4* dv = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.v) + p.mine);
   // behind the sequence's tokens zeros; where there is no such page NaN, so that nobody takes it for a key
   const uint32_t none = p.has ? 0x7fff7fffu : 0u;
   uint4 k[2] = {make_uint4(none, none, none, none), make_uint4(none, none, none, none)}, v[2] = {k[0], k[0]};
-  if constexpr (FORMAT == PI05_CACHE_BF16) {
-    if (p.has && p.good) {
-      k[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.k) + p.pool) + lane);
-      v[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.v) + p.pool) + lane);
-    }
-    __stcs(dk + lane, k[0]);
-    __stcs(dv + lane, v[0]);
-  } else {
-    if (p.has && p.good) {
+  if (p.has && p.good) {
+    if constexpr (FORMAT == PI05_CACHE_BF16) {
+      load_32(k, reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.k) + p.pool) + 2 * lane, a.wide);
+      load_32(v, reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.v) + p.pool) + 2 * lane, a.wide);
+    } else {
       const uint4 kc = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.c.k) + p.pool) + lane);
       const uint4 vc = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.c.v) + p.pool) + lane);
       const float ks = __ldg(a.c.k_scale + p.scale), vs = __ldg(a.c.v_scale + p.scale);
       k[0] = decode<FORMAT>(kc.x, kc.y, ks); k[1] = decode<FORMAT>(kc.z, kc.w, ks);
       v[0] = decode<FORMAT>(vc.x, vc.y, vs); v[1] = decode<FORMAT>(vc.z, vc.w, vs);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      __stcs(dk + 2 * lane + i, k[i]);
-      __stcs(dv + 2 * lane + i, v[i]);
-    }
   }
+  store_32(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.k) + p.mine) + 2 * lane, k, a.wide);
+  store_32(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.r.v) + p.mine) + 2 * lane, v, a.wide);
 }
 
 typedef void (*RowKernel)(const RowArgs);
@@ -213,8 +218,10 @@ int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c,
     return PI05_ERR_ARGUMENT;
   DeviceGuard guard(device);
   if (!guard.ok) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
-  const int per = BLOCK / lanes(c->format, c->head_dim);
-  const RowArgs a = {*c, *r, (unsigned)rows};
+  const int per = BLOCK / (c->head_dim / 16);
+  uintptr_t bits = (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)(2 * (r->batch_stride | r->layer_stride | r->token_stride | r->head_stride));
+  if (c->format == PI05_CACHE_BF16) bits |= (uintptr_t)c->k | (uintptr_t)c->v;
+  const RowArgs a = {*c, *r, (unsigned)rows, (bits & 31) == 0};
   const RowKernel kernel = kernels[c->format][c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2];
   kernel<<<dim3((unsigned)((rows + per - 1) / per), r->layers, r->batch), BLOCK, 0, (cudaStream_t)stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? PI05_OK : PI05_ERR_CUDA;

@@ -172,6 +172,25 @@ def test_strided_inputs_and_outputs():
     assert torch.equal(again[0], k)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_rows_that_begin_on_16_bytes_only(fmt):
+    """Rows at odd multiples of 16 bytes, in and out: the same as aligned ones."""
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randn(2, 1, 7, 3, 136, generator=g).to(torch.bfloat16).cuda()
+    k, v = wide[..., :128], wide[..., 8:]                                 # heads 272 bytes apart; v behind 16
+    c = make(fmt, 3, 1, 16, 3, 128)
+    table = torch.tensor([[2], [1]], dtype=torch.int32, device="cuda")
+    c.write(k, v, table)
+    want = c.read(table, 7)
+    for b, p in enumerate((2, 1)):
+        check_held(c, "k", p, 0, 0, k[b].cpu())
+        check_held(c, "v", p, 0, 0, v[b].cpu())
+    out = torch.zeros(2, 2, 1, 7, 3, 136, dtype=torch.bfloat16, device="cuda")
+    c.read(table, 7, out=(out[0][..., 8:], out[1][..., 8:]))
+    c.status()
+    assert torch.equal(out[0][..., 8:], want[0]) and torch.equal(out[1][..., 8:], want[1]) and bool((out[..., :8] == 0).all())
+
+
 def test_bad_pages_and_positions_are_left_out():
     c = make("int8", 4, 1, 16, 1, 64, fill=0x11)
     k = torch.randn(4, 1, 16, 1, 64).to(torch.bfloat16).cuda()
