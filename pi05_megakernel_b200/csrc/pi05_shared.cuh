@@ -492,23 +492,26 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             }
           }
           const unsigned gone = __ballot_sync(0xffffffffu, bad);
-          uint32_t m0 = 0, m1 = 0;            // lane k: keys of tile i0 + k
-          const bool masked = p.s.prefix_valid && g.first + i0 < p_tiles;
-          uint8_t valid[2 * BATCH];           // (all on their way before the first is looked at)
-#pragma unroll
-          for (int k = 0; k < 2 * BATCH; ++k) {
-            const int i = g.first + i0 + k / 2;
-            const uint32_t key = (uint32_t)i * TILE + (k & 1) * 32 + lane;
-            valid[k] = 1;
-            if (masked && i < p_tiles && key < (uint32_t)p.s.prefix_tokens) valid[k] = __ldcg(p.s.prefix_valid + key);
-          }
-#pragma unroll
-          for (int k = 0; k < BATCH; ++k) {
-            const int i = g.first + i0 + k;
+          // lane k: keys of tile i0 + k that count
+          uint32_t m0, m1;
+          {
+            const int i = g.first + i0 + lane;
             const bool own = i >= p_tiles;
-            const uint32_t key = (uint32_t)(own ? i - p_tiles : i) * TILE + lane, end = i0 + k >= g.n ? 0u : own ? length : (uint32_t)p.s.prefix_tokens;
-            const unsigned w0 = __ballot_sync(0xffffffffu, key < end && valid[2 * k]), w1 = __ballot_sync(0xffffffffu, key + 32 < end && valid[2 * k + 1]);
-            if (lane == k) { m0 = w0; m1 = w1; }
+            const uint32_t key = (uint32_t)(own ? i - p_tiles : i) * TILE, end = own ? length : (uint32_t)p.s.prefix_tokens;
+            const uint32_t left = end > key ? end - key : 0u;
+            m0 = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+            m1 = left >= 64 ? 0xffffffffu : left > 32 ? (1u << (left - 32)) - 1u : 0u;
+          }
+          if (p.s.prefix_valid && g.first + i0 < p_tiles) {
+            // a lane looks sixteen keys up, all on their way at once
+            const uint32_t key = (uint32_t)(g.first + i0) * TILE + 16 * lane, end = p.s.prefix_tokens;
+            uint32_t bits = 0;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) bits |= (key + k >= end || __ldcg(p.s.prefix_valid + key + k) ? 1u : 0u) << k;
+            const int from = 4 * (lane & 7);
+            const uint32_t a = __shfl_sync(0xffffffffu, bits, from), b = __shfl_sync(0xffffffffu, bits, from + 1), c = __shfl_sync(0xffffffffu, bits, from + 2),
+                           d = __shfl_sync(0xffffffffu, bits, from + 3);
+            if (g.first + i0 + lane < p_tiles) { m0 &= a | b << 16; m1 &= c | d << 16; }
           }
 #pragma unroll 1
           for (int k = 0; k < BATCH && i0 + k < g.n && ok; ++k) {
@@ -519,13 +522,12 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             const int j = lane - k * pieces;
             if (j >= 0 && j < pieces) { info.page[j] = page; info.in[j] = in; }
             if (lane == k) {
-              uint32_t b0 = 0, b1 = 0;
-              for (int q = 0; q < pieces; ++q)
-                if (gone >> (k * pieces + q) & 1) {
-                  const unsigned long long keys = (p.piece == 64 ? ~0ull : (1ull << p.piece) - 1) << (q * p.piece);
-                  b0 |= (uint32_t)keys;
-                  b1 |= (uint32_t)(keys >> 32);
-                }
+              unsigned long long lost = 0;
+              if (gone)
+#pragma unroll 1
+                for (int q = 0; q < pieces; ++q)
+                  if (gone >> (k * pieces + q) & 1) lost |= (p.piece == 64 ? ~0ull : (1ull << p.piece) - 1) << (q * p.piece);
+              const uint32_t b0 = (uint32_t)lost, b1 = (uint32_t)(lost >> 32);
               info.mask[0] = m0; info.mask[1] = m1; info.bad[0] = b0 & m0; info.bad[1] = b1 & m1;
             }
             __syncwarp();
@@ -829,7 +831,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
     // neighbouring lanes take 64 bytes of an even row and the other 64 of the odd one, so that neither the loads nor the stores share banks
     const int group = (warp - 12) >> 2, w = warp & 3, odd = lane >> 2 & 1, chunk = lane & 3, high = lane >> 3;
     const int blk = BLOCKS == 4 ? high ^ odd : BLOCKS == 2 ? (high & 1) ^ odd : 0;
-    constexpr int AT_ONCE = 8 / BLOCKS;     // rows of a warp's turn
+    constexpr int ROWS_AT_ONCE = 8 / BLOCKS;         // rows of a warp's turn
     const int first = odd + (BLOCKS == 4 ? 0 : BLOCKS == 2 ? (high >> 1) * 2 : high * 2);
     uint32_t unit = 0;
     while (ok && NEXT) {
@@ -841,22 +843,20 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         ok = WAIT(raw_full + 8 * from, (n / RAW) & 1, WAIT_RAW_FULL);
         if (ok && n >= UNITS) ok = WAIT(kv_empty + 8 * to, (n / UNITS - 1) & 1, WAIT_KV_EMPTY);
         if (!ok) break;
-        constexpr int TURNS = TILE / AT_ONCE / 4;
-        uint4 x[TURNS];
-#pragma unroll
-        for (int j = 0; j < TURNS; ++j) x[j] = ptx::ld_shared_v4(raw + from * RAW_UNIT + ((j * 4 + w) * AT_ONCE + first) * DIM + blk * 64 + chunk * 16);
-        auto turn = [&](auto value) {
-#pragma unroll
+        constexpr int TURNS = TILE / ROWS_AT_ONCE / 4;
+        auto turns = [&](auto value) {
+#pragma unroll 2
           for (int j = 0; j < TURNS; ++j) {
-            const int r = (j * 4 + w) * AT_ONCE + first;
-            const uint2 a = value(x[j].x), c = value(x[j].y), d = value(x[j].z), e = value(x[j].w);
+            const int r = (j * 4 + w) * ROWS_AT_ONCE + first;
+            const uint4 x = ptx::ld_shared_v4(raw + from * RAW_UNIT + r * DIM + blk * 64 + chunk * 16);
+            const uint2 a = value(x.x), c = value(x.y), d = value(x.z), e = value(x.w);
             const uint32_t line = ring + to * UNIT + blk * (TILE * 128) + r * 128;
             ptx::st_shared_v4(line + (((2 * chunk) ^ (r & 7)) << 4), a.x, a.y, c.x, c.y);
             ptx::st_shared_v4(line + (((2 * chunk + 1) ^ (r & 7)) << 4), d.x, d.y, e.x, e.y);
           }
         };
-        if (is_v) turn([](uint32_t c) { return cache::quad_half<FORMAT>(c); });
-        else turn([](uint32_t c) { return cache::quad<FORMAT>(c); });
+        if (is_v) turns([](uint32_t c) { return cache::quad_half<FORMAT>(c); });
+        else turns([](uint32_t c) { return cache::quad<FORMAT>(c); });
         ptx::fence_proxy_async_shared();
         __syncwarp();
         if (lane == 0) { ptx::mbar_arrive(kv_full + 8 * to); ptx::mbar_arrive(raw_empty + 8 * from); }
