@@ -33,7 +33,10 @@ constexpr int TILE = 64;                    // keys of a tile
 constexpr int ROWS = 128;                   // query rows of a tile
 constexpr int INFO = 16;                    // tiles that pages and masks are looked up ahead, in
 constexpr int BATCH = 8;                    // rounds of
-constexpr int OVERHEAD = 2;                 // what an item costs beside its tiles: loading Q, storing O
+// What an item costs beside its tiles (loading Q, filling the pipeline, storing O), in tiles, by what the CTAs of one launch measured: with 2 for an 8-bit cache those with
+// nothing but short items took half as long again as the others.  Drafts (32 x 8 over 8192, e4m3): 170 us with 2, 140 with 4, 133 with 6; 64 sequences over
+// 16384 (BF16): 79.7 with 2, 77.8 with 3, 80.2 with 4.
+__host__ __device__ constexpr int overhead(int format) { return format == PI05_CACHE_BF16 ? 3 : 5; }
 constexpr int MAX_BATCH = 1024;
 constexpr float RESCALE = 8.0f;             // of exponents to the base 2: probabilities up to 256, their sums far from the ends of FP32
 
@@ -62,6 +65,7 @@ struct Args {
   float c_log2;                             // scale x log2 e
   int2* parts;                              // of every item, the batch's before the sequences': its first slot, and how many there are (0 or 1 that was finished: none to add)
   float *a_parts, *b_parts;                 // slots of unfinished items: [D / 4][rows][4], then (reference, weight) per row
+  int overhead;                             // units of an item beside its tiles
   uint32_t limit;                           // of a wait, in cycles
 };
 
@@ -93,7 +97,7 @@ struct Walk {
   }
   __device__ __forceinline__ void set(const Args& p, const int* s) {
     sums = s;
-    a_cost = OVERHEAD + p.p_tiles;
+    a_cost = p.overhead + p.p_tiles;
     a_units = p.joined ? 0 : a_cost * p.a_tiles * p.c.kv_heads;
     b_units = s[p.s.batch];
     const int u = a_units + b_units * p.c.kv_heads;
@@ -134,11 +138,11 @@ static __device__ __noinline__ int next_segment(const Args& p, const Walk& w, in
       g.r = 0;
       if (p.b_tiles > 1) { cost /= p.b_tiles; g.r = off / cost; off -= g.r * cost; }
       g.item = (g.h * p.s.batch + g.b) * p.b_tiles + g.r;
-      g.tiles = cost - OVERHEAD;
+      g.tiles = cost - p.overhead;
     }
     const int last = off + (end - at) < cost ? off + (end - at) : cost;      // units of the item before `end`
-    g.first = off > OVERHEAD ? off - OVERHEAD : 0;
-    g.n = last - OVERHEAD - g.first;
+    g.first = off > p.overhead ? off - p.overhead : 0;
+    g.n = last - p.overhead - g.first;
     at += last - off;
   }
   __syncwarp();
@@ -173,12 +177,12 @@ __device__ __forceinline__ int own_length(const Args& p, int b) {
 
 // Four MMAs of K = 16, the A operand from tensor memory, B from shared memory: 8 columns and STEP descriptor units further each.
 template <int STEP>
-__device__ __forceinline__ void umma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t accumulate, uint32_t on) {
-#define PI05_UMMA1(P0) "mov.b64 db, {bl, %6};\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [aa], db, %3, " P0 ";\n"
-#define PI05_UMMA_STEP "add.u32 bl, bl, %7;\n add.u32 aa, aa, 8;\n"
-  asm volatile("{\n.reg .pred p, q, t;\n.reg .b32 aa, bl;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\nsetp.eq.b32 t, 0, 0;\n"
+__device__ __forceinline__ void umma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+#define PI05_UMMA1(P0) "mov.b64 db, {bl, %5};\ntcgen05.mma.cta_group::1.kind::f16 [%0], [aa], db, %3, " P0 ";\n"
+#define PI05_UMMA_STEP "add.u32 bl, bl, %6;\n add.u32 aa, aa, 8;\n"
+  asm volatile("{\n.reg .pred p, t;\n.reg .b32 aa, bl;\n.reg .b64 db;\nsetp.ne.b32 p, %4, 0;\nsetp.eq.b32 t, 0, 0;\n"
                "mov.b32 aa, %1;\nmov.b32 bl, %2;\n" PI05_UMMA1("p") PI05_UMMA_STEP PI05_UMMA1("t") PI05_UMMA_STEP PI05_UMMA1("t") PI05_UMMA_STEP PI05_UMMA1("t") "}"
-               ::"r"(d), "r"(a), "r"(blo), "r"(idesc), "r"(accumulate), "r"(on), "n"(ptx::UMMA_DESC_HI), "n"(STEP) : "memory");
+               ::"r"(d), "r"(a), "r"(blo), "r"(idesc), "r"(accumulate), "n"(ptx::UMMA_DESC_HI), "n"(STEP) : "memory");
 #undef PI05_UMMA1
 #undef PI05_UMMA_STEP
 }
@@ -234,21 +238,39 @@ __device__ __forceinline__ bool wait(const Args& p, uint32_t bar, uint32_t parit
   return __all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity)) || wait_slow(p, bar, parity, kind);
 }
 
+// The same for one thread of a warp.
+static __device__ __noinline__ bool wait_one_slow(const Args& p, uint32_t bar, uint32_t parity, int kind) {
+  const uint32_t t0 = (uint32_t)clock();
+#pragma unroll 1
+  do {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+  } while ((uint32_t)clock() - t0 <= p.limit);
+  if (atomicCAS(p.c.status + 2, 0u, (unsigned)kind) == 0u) p.c.status[3] = blockIdx.x << 16;
+  const uint32_t t1 = (uint32_t)clock();
+  while ((uint32_t)clock() - t1 < 200000u) __nanosleep(1000);
+  return false;
+}
+__device__ __forceinline__ bool wait_one(const Args& p, uint32_t bar, uint32_t parity, int kind) {
+  return ptx::mbar_try_wait(bar, parity) || wait_one_slow(p, bar, parity, kind);
+}
+
 // The queries of a softmax warp's 32 rows, as they lie, into tensor memory.
 template <int DIM>
 __device__ __noinline__ void load_queries(const Args& p, const Segment& s, int row, uint32_t columns) {
   int b = 0, t = 0, head = 0;
   const bool mine = row_of(p, s, row, b, t, head);
   const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.s.q) + b * p.s.q_batch_stride + t * p.s.q_token_stride + head * p.s.q_head_stride);
+  constexpr int WORDS = DIM >= 128 ? 64 : 32;                      // on their way at once
 #pragma unroll 1
-  for (int c = 0; c < DIM / 64; ++c) {
-    uint32_t w[32];
+  for (int c = 0; c < DIM / 2; c += WORDS) {
+    uint32_t w[WORDS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint4 x = mine ? __ldcg(q + c * 8 + j) : make_uint4(0u, 0u, 0u, 0u);
+    for (int j = 0; j < WORDS / 4; ++j) {
+      const uint4 x = mine ? __ldcg(q + c / 4 + j) : make_uint4(0u, 0u, 0u, 0u);
       w[4 * j] = x.x; w[4 * j + 1] = x.y; w[4 * j + 2] = x.z; w[4 * j + 3] = x.w;
     }
-    tmem_st_32x32(columns + 32 * c, w);
+#pragma unroll
+    for (int j = 0; j < WORDS; j += 32) tmem_st_32x32(columns + c + j, reinterpret_cast<uint32_t(&)[32]>(w[j]));
   }
   ptx::tmem_wait_st();
   ptx::tc_fence_before();
@@ -260,6 +282,8 @@ struct Info {
   uint32_t mask[2];                         // keys that count
   uint32_t bad[2];                          // keys of pages that do not exist
   int page[4], in[4];                       // page and place of the tile's pieces; page -1: nothing to copy
+  long long scale[4];                       // of their first scales
+  int there;                                // pieces to copy
 };
 
 template <int FORMAT, int DIM>
@@ -298,6 +322,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
                  s_full = take(S_BUFS), s_free = take(S_BUFS), p_full = take(2), pv_done = take(2);
   const bool leader = ptx::elect_one();
 #define WAIT(BAR, PARITY, KIND) wait(p, BAR, PARITY, KIND)
+#define WAIT_ONE(BAR, PARITY, KIND) wait_one(p, BAR, PARITY, KIND)
 
   if (CODES && tid < TILE) s_ones[tid] = 1.f;
   if (warp == 0) {
@@ -324,7 +349,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         if (blockIdx.x == 0 && p.s.table && __ldcg(p.s.lengths + b) != n) cache::report(p.c.status, cache::BAD_POSITION, b);
         lengths[b] = n;
         const int tiles = (p.joined ? p.p_tiles : 0) + (n + TILE - 1) / TILE;
-        cost = tiles ? (OVERHEAD + tiles) * p.b_tiles : 0;
+        cost = tiles ? (p.overhead + tiles) * p.b_tiles : 0;
       }
       for (int d = 1; d < 32; d <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, cost, d);
@@ -342,31 +367,6 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   ptx::grid_dep_launch();
   const uint32_t tmem = s_tmem;
   const Walk& walk = s_walk;
-  // What the combine kernel has to know of the items: the slots of their parts
-  {
-    const int a_items = p.joined ? 0 : p.a_tiles * p.c.kv_heads, items = a_items + p.s.batch * p.c.kv_heads * p.b_tiles;
-    for (int item = tid * gridDim.x + blockIdx.x; item < items; item += gridDim.x * blockDim.x) {
-      int at = 0, tiles = 0;                // first unit behind the item's overhead
-      const int own = item - a_items;
-      if (own < 0) {
-        at = item * walk.a_cost;
-        tiles = p.p_tiles;
-      } else {
-        const int hb = own / p.b_tiles, h = hb / p.s.batch, b = hb - h * p.s.batch, units = sums[b + 1] - sums[b];
-        if (units) {
-          const int cost = units / p.b_tiles;
-          at = walk.a_units + h * walk.b_units + sums[b] + (own - hb * p.b_tiles) * cost;
-          tiles = cost - OVERHEAD;
-        }
-      }
-      int2 part = make_int2(0, 0);
-      if (tiles) {
-        const int first = walk.cta_of(at + OVERHEAD), n = walk.cta_of(at + OVERHEAD + tiles - 1) - first + 1;
-        part = make_int2(first + (own < 0 ? item : own), own >= 0 && p.joined && n == 1 ? -1 : n);
-      }
-      p.parts[item] = part;
-    }
-  }
   // Where the keys and values of a segment's tile i of n stand among the segment's units, which is the order of their use: LOOK = 1: K0, K1, V0,
   // K2, V1, .., V(n-1); 2: K0, K1, K2, V0, K3, V1, .., V(n-2), V(n-1).  And what unit u is.
   auto k_unit = [](int i) { return i < LOOK ? i : 2 * i - LOOK; };
@@ -384,85 +384,95 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
 
   if (warp < 4) {
     if (warp == 0) {
-      // ---- copies, a lane each
+      // ---- copies, by one thread
       uint32_t unit = 0, tile = 0;            // of all segments
-      const int pieces = TILE / p.piece, copies = CODES || p.piece == TILE ? pieces : pieces * BLOCKS, j = lane % pieces, blk = lane / pieces;
+      const int pieces = TILE / p.piece;
       ptx::grid_dep_wait();
       while (ok && NEXT) {
+        if (leader) {
+          const int units_here = 2 * g.n, h = g.h;
 #pragma unroll 1
-        for (int u = 0; u < 2 * g.n && ok; ++u, ++unit) {
-          bool is_v;
-          const uint32_t n = tile + what(u, g.n, is_v), slot = n % INFO;
-          if (!is_v) ok = WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
-          constexpr int RING = CODES ? RAW : UNITS;
-          const uint32_t at = unit % RING, round = unit / RING, full = (CODES ? raw_full : kv_full) + 8 * at;
-          if (ok && round) ok = WAIT((CODES ? raw_empty : kv_empty) + 8 * at, (round - 1) & 1, CODES ? WAIT_RAW_EMPTY : WAIT_KV_EMPTY);
-          if (!ok) break;
-          const int page = s_info[slot].page[j], in = s_info[slot].in[j];
-          const int there = __popc(__ballot_sync(0xffffffffu, lane < pieces && page >= 0));
-          if (leader) {
-            ptx::mbar_expect_tx(full, there * p.piece * DIM * (CODES ? 1 : 2));
-            if (CODES && !is_v) ptx::mbar_expect_tx(scale_full + 8 * slot, there * p.piece * 8);
-          }
-          __syncwarp();
-          const CUtensorMap* map = is_v ? &p.v : &p.k;
-          if constexpr (CODES) {
-            const uint32_t dst = raw + at * RAW_UNIT;
-            if (lane < pieces && page >= 0) ptx::tma_load_4d(dst + j * p.piece * DIM, map, full, 0, in, g.h, page);
-            __syncwarp();
-            if (!is_v && lane < 2 * pieces && page >= 0) {           // a piece's scales: of the keys, of the values
-              const long long sc = (((long long)page * p.c.layers + p.s.layer) * p.c.kv_heads + g.h) * p.c.page_tokens + in;
-              bulk_load(scales + ((slot * 2 + blk) * TILE + j * p.piece) * 4, (blk ? p.c.v_scale : p.c.k_scale) + sc, p.piece * 4, scale_full + 8 * slot);
+          for (int u = 0; u < units_here; ++u, ++unit) {
+            bool is_v;
+            const uint32_t n = tile + what(u, g.n, is_v), slot = n % INFO;
+            constexpr int RING = CODES ? RAW : UNITS;
+            const uint32_t at = unit % RING, round = unit / RING, full = (CODES ? raw_full : kv_full) + 8 * at;
+            if (!is_v) ok = WAIT_ONE(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
+            if (ok && round) ok = WAIT_ONE((CODES ? raw_empty : kv_empty) + 8 * at, (round - 1) & 1, CODES ? WAIT_RAW_EMPTY : WAIT_KV_EMPTY);
+            if (!ok) break;
+            const Info& info = s_info[slot];
+            const int there = info.there * p.piece;
+            const CUtensorMap* map = is_v ? &p.v : &p.k;
+            const uint32_t dst = CODES ? raw + at * RAW_UNIT : ring + at * UNIT;
+            ptx::mbar_expect_tx(full, there * DIM * (CODES ? 1 : 2));
+            if (CODES && !is_v) ptx::mbar_expect_tx(scale_full + 8 * slot, there * 8);
+#pragma unroll 1
+            for (int j = 0; j < pieces; ++j) {
+              const int page = info.page[j], in = info.in[j];
+              if (page < 0) continue;
+              if constexpr (CODES) {
+                ptx::tma_load_4d(dst + j * p.piece * DIM, map, full, 0, in, h, page);
+                if (!is_v) {
+                  const uint32_t to = scales + (slot * 2 * TILE + j * p.piece) * 4;
+                  bulk_load(to, p.c.k_scale + info.scale[j], p.piece * 4, scale_full + 8 * slot);
+                  bulk_load(to + TILE * 4, p.c.v_scale + info.scale[j], p.piece * 4, scale_full + 8 * slot);
+                }
+              } else if (pieces == 1) {
+                ptx::tma_load_5d(dst, map, full, 0, in, 0, h, page);
+              } else {
+#pragma unroll 1
+                for (int blk = 0; blk < BLOCKS; ++blk) ptx::tma_load_5d(dst + blk * TILE * 128 + j * p.piece * 128, map, full, 0, in, blk, h, page);
+              }
             }
-          } else {
-            const uint32_t dst = ring + at * UNIT;
-            if (lane < copies && page >= 0) ptx::tma_load_5d(dst + blk * TILE * 128 + j * p.piece * 128, map, full, 0, in, blk, g.h, page);
+            if (is_v) ptx::mbar_arrive(info_empty + 8 * slot);
           }
-          __syncwarp();
-          if (is_v && leader) ptx::mbar_arrive(info_empty + 8 * slot);
-          __syncwarp();
         }
+        __syncwarp();
+        ok = __any_sync(0xffffffffu, leader && ok);
         tile += g.n;
       }
     } else if (warp == 1) {
-      // ---- MMAs
-      const uint32_t on = leader ? 1u : 0u;
+      // ---- MMAs, by one thread
       const uint32_t idesc_s = ptx::umma_idesc_bf16(ROWS, TILE);
       const uint32_t idesc_o = (ptx::umma_idesc_bf16(ROWS, DIM) & (CODES ? ~((1u << 7) | (1u << 10)) : ~0u)) | ptx::UMMA_B_MN_MAJOR;     // (FP16 is type 0)
       const uint32_t kdesc = (uint32_t)ptx::umma_smem_desc(ring), vdesc = (uint32_t)ptx::umma_smem_desc_mn(ring, TILE * 128);
       uint32_t unit = 0, tile = 0, seg = 0;
       while (ok && NEXT) {
-        ok = WAIT(q_full + 8 * (seg % Q_BUFS), (seg / Q_BUFS) & 1, WAIT_Q);
-        ptx::tc_fence_after();
-        const uint32_t q = tmem + TM_Q + seg % Q_BUFS * (DIM / 2);
+        if (leader) {
+          ok = WAIT_ONE(q_full + 8 * (seg % Q_BUFS), (seg / Q_BUFS) & 1, WAIT_Q);
+          ptx::tc_fence_after();
+          const uint32_t q = tmem + TM_Q + seg % Q_BUFS * (DIM / 2);
+          const int count = g.n;
 #pragma unroll 1
-        for (int i = 0; i < g.n + LOOK && ok; ++i) {
-          if (i < g.n) {
-            const uint32_t n = tile + i, buf = n % S_BUFS, u = unit + k_unit(i), at = u % UNITS;
-            if (OVER && n > 1) ok = WAIT(pv_done + 8 * buf, ((n >> 1) - 1) & 1, WAIT_PV);
-            if (!OVER && n >= S_BUFS) ok = WAIT(s_free + 8 * buf, (n / S_BUFS - 1) & 1, WAIT_S_FREE);
-            if (ok) ok = WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            const uint32_t kd = kdesc + at * (UNIT >> 4);
+          for (int i = 0; i < count + LOOK && ok; ++i) {
+            if (i < count) {
+              const uint32_t n = tile + i, buf = n % S_BUFS, u = unit + k_unit(i), at = u % UNITS;
+              if (OVER && n > 1) ok = WAIT_ONE(pv_done + 8 * buf, ((n >> 1) - 1) & 1, WAIT_PV);
+              if (!OVER && n >= S_BUFS) ok = WAIT_ONE(s_free + 8 * buf, (n / S_BUFS - 1) & 1, WAIT_S_FREE);
+              if (ok) ok = WAIT_ONE(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              const uint32_t kd = kdesc + at * (UNIT >> 4);
 #pragma unroll
-            for (int j = 0; j < BLOCKS; ++j) umma_ts4<2>(tmem + TM_S + buf * TILE, q + 32 * j, kd + j * (TILE * 128 >> 4), idesc_s, j ? 1u : 0u, on);
-            if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(s_full + 8 * buf); }
-            __syncwarp();
-          }
-          if (i >= LOOK) {
-            const uint32_t n = tile + i - LOOK, buf = n & 1, u = unit + v_unit(i - LOOK, g.n), at = u % UNITS;
-            if (i == LOOK && seg) ok = WAIT(o_free, (seg - 1) & 1, WAIT_O_FREE);
-            if (ok) ok = WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
-            if (ok) ok = WAIT(p_full + 8 * buf, (n >> 1) & 1, WAIT_P);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            const uint32_t vd = vdesc + at * (UNIT >> 4);
-            umma_ts4<(16 * 128 >> 4)>(tmem + TM_O, tmem + TM_P + buf * P_STEP, vd, idesc_o, i > LOOK ? 1u : 0u, on);
-            if (leader) { ptx::umma_commit(kv_empty + 8 * at); ptx::umma_commit(pv_done + 8 * buf); }
-            __syncwarp();
+              for (int j = 0; j < BLOCKS; ++j) umma_ts4<2>(tmem + TM_S + buf * TILE, q + 32 * j, kd + j * (TILE * 128 >> 4), idesc_s, j ? 1u : 0u);
+              ptx::umma_commit(kv_empty + 8 * at);
+              ptx::umma_commit(s_full + 8 * buf);
+            }
+            if (i >= LOOK) {
+              const uint32_t n = tile + i - LOOK, buf = n & 1, u = unit + v_unit(i - LOOK, count), at = u % UNITS;
+              if (i == LOOK && seg) ok = WAIT_ONE(o_free, (seg - 1) & 1, WAIT_O_FREE);
+              if (ok) ok = WAIT_ONE(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
+              if (ok) ok = WAIT_ONE(p_full + 8 * buf, (n >> 1) & 1, WAIT_P);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              umma_ts4<(16 * 128 >> 4)>(tmem + TM_O, tmem + TM_P + buf * P_STEP, vdesc + at * (UNIT >> 4), idesc_o, i > LOOK ? 1u : 0u);
+              ptx::umma_commit(kv_empty + 8 * at);
+              ptx::umma_commit(pv_done + 8 * buf);
+            }
           }
         }
+        __syncwarp();
+        ok = __any_sync(0xffffffffu, leader && ok);
         unit += 2 * g.n;
         tile += g.n;
         ++seg;
@@ -478,7 +488,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         for (int i0 = 0; i0 < g.n && ok; i0 += BATCH) {
           // this lane's piece of tile i0 + lane / pieces
           int page = -1, in = 0;
-          bool bad = false;
+          int looked = 0;                     // 1: in the prefix's table, 2: in the sequence's
           {
             const int i = g.first + i0 + lane / pieces;
             const bool own = i >= p_tiles;
@@ -487,11 +497,20 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
               const uint32_t lp = first / (uint32_t)p.c.page_tokens;
               in = (int)(first - lp * (uint32_t)p.c.page_tokens);
               page = __ldcg((own ? p.s.table + (long long)g.b * p.s.table_stride : p.s.prefix_table) + lp);
-              bad = page < 0 || page >= p.c.pages;
-              if (bad) { page = -1; cache::report(p.c.status, cache::BAD_PAGE, own ? g.b : -1); }
+              looked = own ? 2 : 1;
             }
           }
+          uint32_t bits = 0;                  // sixteen keys of the prefix a lane, on their way together with the pages
+          const bool masked = p.s.prefix_valid && g.first + i0 < p_tiles;
+          if (masked) {
+            const uint32_t key = (uint32_t)(g.first + i0) * TILE + 16 * lane, end = p.s.prefix_tokens;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) bits |= (key + k >= end || __ldcg(p.s.prefix_valid + key + k) ? 1u : 0u) << k;
+          }
+          const bool bad = looked && (page < 0 || page >= p.c.pages);
+          if (bad) { page = -1; cache::report(p.c.status, cache::BAD_PAGE, looked == 2 ? g.b : -1); }
           const unsigned gone = __ballot_sync(0xffffffffu, bad);
+          const long long scale = (((long long)page * p.c.layers + p.s.layer) * p.c.kv_heads + g.h) * p.c.page_tokens + in;
           // lane k: keys of tile i0 + k that count
           uint32_t m0, m1;
           {
@@ -502,12 +521,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             m0 = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
             m1 = left >= 64 ? 0xffffffffu : left > 32 ? (1u << (left - 32)) - 1u : 0u;
           }
-          if (p.s.prefix_valid && g.first + i0 < p_tiles) {
-            // a lane looks sixteen keys up, all on their way at once
-            const uint32_t key = (uint32_t)(g.first + i0) * TILE + 16 * lane, end = p.s.prefix_tokens;
-            uint32_t bits = 0;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) bits |= (key + k >= end || __ldcg(p.s.prefix_valid + key + k) ? 1u : 0u) << k;
+          if (masked) {
             const int from = 4 * (lane & 7);
             const uint32_t a = __shfl_sync(0xffffffffu, bits, from), b = __shfl_sync(0xffffffffu, bits, from + 1), c = __shfl_sync(0xffffffffu, bits, from + 2),
                            d = __shfl_sync(0xffffffffu, bits, from + 3);
@@ -520,7 +534,8 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             if (!ok) break;
             Info& info = s_info[slot];
             const int j = lane - k * pieces;
-            if (j >= 0 && j < pieces) { info.page[j] = page; info.in[j] = in; }
+            if (j >= 0 && j < pieces) { info.page[j] = page; info.in[j] = in; info.scale[j] = scale; }
+            const int there = __popc(__ballot_sync(0xffffffffu, j >= 0 && j < pieces && page >= 0));
             if (lane == k) {
               unsigned long long lost = 0;
               if (gone)
@@ -528,6 +543,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
                 for (int q = 0; q < pieces; ++q)
                   if (gone >> (k * pieces + q) & 1) lost |= (p.piece == 64 ? ~0ull : (1ull << p.piece) - 1) << (q * p.piece);
               const uint32_t b0 = (uint32_t)lost, b1 = (uint32_t)(lost >> 32);
+              info.there = there;
               info.mask[0] = m0; info.mask[1] = m1; info.bad[0] = b0 & m0; info.bad[1] = b1 & m1;
             }
             __syncwarp();
@@ -538,6 +554,31 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         tile += g.n;
       }
     } else if (warp == 3) {
+      // What the combine kernel has to know of the items: the slots of their parts
+      {
+        const int a_items = p.joined ? 0 : p.a_tiles * p.c.kv_heads, items = a_items + p.s.batch * p.c.kv_heads * p.b_tiles;
+        for (int item = lane * gridDim.x + blockIdx.x; item < items; item += gridDim.x * 32) {
+          int at = 0, tiles = 0;                // first unit behind the item's overhead
+          const int own = item - a_items;
+          if (own < 0) {
+            at = item * walk.a_cost;
+            tiles = p.p_tiles;
+          } else {
+            const int hb = own / p.b_tiles, h = hb / p.s.batch, b = hb - h * p.s.batch, units = sums[b + 1] - sums[b];
+            if (units) {
+              const int cost = units / p.b_tiles;
+              at = walk.a_units + h * walk.b_units + sums[b] + (own - hb * p.b_tiles) * cost;
+              tiles = cost - p.overhead;
+            }
+          }
+          int2 part = make_int2(0, 0);
+          if (tiles) {
+            const int first = walk.cta_of(at + p.overhead), n = walk.cta_of(at + p.overhead + tiles - 1) - first + 1;
+            part = make_int2(first + (own < 0 ? item : own), own >= 0 && p.joined && n == 1 ? -1 : n);
+          }
+          p.parts[item] = part;
+        }
+      }
       // ---- the largest scale of a tile's values that count
       if constexpr (CODES) {
         uint32_t tile = 0;
@@ -610,11 +651,8 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
 #pragma unroll 1
       for (int i = (tile & 1) ^ group; i < count; i += 2) {
         const uint32_t n = tile + i, buf = group, sbuf = n % S_BUFS, slot = n % INFO;
-        ok = ok && WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
-        if (CODES) {
-          ok = ok && WAIT(scale_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
-          ok = ok && WAIT(vlog_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
-        }
+        // (warp 3 has waited for the tile's masks and scales before it reports)
+        ok = ok && WAIT((CODES ? vlog_full : info_full) + 8 * slot, (n / INFO) & 1, CODES ? WAIT_SCALES : WAIT_INFO);
         const uint32_t mask0 = s_info[slot].mask[0], mask1 = s_info[slot].mask[1];
         const uint32_t bad0 = CODES ? s_bad[slot][0] : s_info[slot].bad[0], bad1 = CODES ? s_bad[slot][1] : s_info[slot].bad[1];
         uint32_t k0 = mask0, k1 = mask1;    // keys that count for this row
@@ -866,6 +904,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
     }
   }
 #undef WAIT
+#undef WAIT_ONE
 #undef NEXT
   ptx::tc_fence_before();
   __syncthreads();
