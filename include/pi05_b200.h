@@ -384,6 +384,14 @@ typedef struct pi05_shared_call {
 int pi05_shared_workspace(int sms, const pi05_cache* cache, int q_heads, int max_batch, int max_tokens, size_t* bytes);
 int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared_call* call, void* workspace, size_t workspace_bytes, void* stream);
 
+/* New tokens of several sequences behind a cached prefix through the layers of the prefill (its handle and weights): per layer the tokens' keys and
+ * values go into the cache (layer by layer, at starts[b] .. of sequence b's pages) and the queries attend to the shared prefix and their sequence's
+ * own tokens there.  embeddings and hidden [batch][tokens][2048] BF16 (hidden: the residual stream behind layer n_layers - 1, before the final
+ * norm); positions [batch][tokens]: of the rotary embedding; `call` gives batch, tokens, tables, lengths (starts[b] + tokens), prefix and causality,
+ * the rest of it is filled in.  batch x tokens is at most the handle's max_tokens; the cache has one KV head of 256 and at least n_layers layers. */
+int pi05_prefill_step(pi05_prefill_t h, const pi05_cache* cache, const pi05_shared_call* call, const void* embeddings, const int* positions,
+                      const int* starts, void* hidden, int n_layers, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

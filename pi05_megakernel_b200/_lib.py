@@ -136,6 +136,8 @@ SIGNATURES = {
     "pi05_cache_status": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
     "pi05_shared_workspace": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
     "pi05_shared_attention": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "pi05_prefill_step": (_c.c_int, [_c.c_void_p, _c.POINTER(Cache), _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int,
+                                     _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "pi05_tuning_defaults": (_c.c_int, [_c.POINTER(Tuning)]),
     "pi05_tune": (_c.c_int, [_c.c_void_p, _c.POINTER(Tuning)]),
     "pi05_chunk_static": (_c.c_int, [_c.c_int, _c.POINTER(_c.c_void_p), _c.c_int, _c.c_void_p, _c.c_int, _c.c_int,

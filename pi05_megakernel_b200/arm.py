@@ -18,6 +18,7 @@ import json
 import torch
 
 from . import _lib
+from .cache import KvCache, check_table
 from .fixture import OBSERVATION, ORDER, Geometry, shapes
 
 
@@ -71,6 +72,17 @@ class PagedPrefix:
         return view, table
 
 
+class CachedPrefix:
+    """The prefix cache in the pages of a ``KvCache`` of 18 layers and one KV head of 256, of any format: every launch reads it back to BF16 first
+    (what the pages and the table hold then).  ``table`` is an int32 tensor ``[batch, pages]`` on the cache's device."""
+
+    def __init__(self, cache: KvCache, table: torch.Tensor) -> None:
+        if cache.kv_heads != 1 or cache.head_dim != 256:
+            raise ValueError("the cache must have one KV head of 256")
+        check_table("table", table, cache.device, 2)
+        self.cache, self.table = cache, table
+
+
 class Pi05Arm:
     name = "b200-megakernel"
 
@@ -109,16 +121,27 @@ class Pi05Arm:
         shape = (geo.horizon, geo.action_dim) if batch == 1 else (batch, geo.horizon, geo.action_dim)
         self.actions = torch.zeros(shape, dtype=torch.float32, device=self.device)
         self.tensors: list[torch.Tensor] | None = None
+        self.cached: tuple[CachedPrefix, tuple[torch.Tensor, torch.Tensor]] | None = None
         self.stamps: torch.Tensor | None = None
         self.config = json.loads(self.lib.pi05_config_json(handle).decode())
         self.config.update(prefix=geo.prefix, steps=self.steps, layers=self.layers, batch=batch)
 
     # ------------------------------------------------------------------ arm protocol
-    def bind(self, inputs: dict, kv_pages: "PagedPrefix | None" = None) -> None:
+    def bind(self, inputs: dict, kv_pages: "PagedPrefix | CachedPrefix | None" = None) -> None:
         """Record the 25 tensors (kept by pointer, read in place).  With ``kv_pages`` the prefix keys / values are read
-        where their producer left them (a strided or paged pool, see ``PagedPrefix``) and ``inputs["prefix_k"]`` /
-        ``inputs["prefix_v"]`` are not needed."""
+        where their producer left them (a strided or paged pool, see ``PagedPrefix``; a quantised cache, see ``CachedPrefix``) and
+        ``inputs["prefix_k"]`` / ``inputs["prefix_v"]`` are not needed."""
         want = shapes(self.geo)
+        cached = None
+        if isinstance(kv_pages, CachedPrefix):
+            cached, kv_pages = kv_pages, None
+            c = cached.cache
+            if c.device != self.device or c.layers != self.geo.layers or cached.table.shape[0] != self.batch or \
+                    cached.table.shape[1] * c.page_tokens < self.geo.prefix:
+                raise ValueError(f"the cache must live on {self.device} and hold {self.geo.layers} layers of {self.geo.prefix} tokens for every observation")
+            shape = (self.batch, *want["prefix_k"][0])
+            dense = tuple(torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+            inputs = {**inputs, "prefix_k": dense[0] if self.batch > 1 else dense[0][0], "prefix_v": dense[1] if self.batch > 1 else dense[1][0]}
         tensors = []
         for name in ORDER:
             if kv_pages is not None and name in ("prefix_k", "prefix_v"):
@@ -148,6 +171,7 @@ class Pi05Arm:
             tensors += [kv_pages.k, kv_pages.v]
             del keep
         self.tensors = tensors
+        self.cached = None if cached is None else (cached, dense)
         # the engine chooses its schedule when it knows the batch: record what it chose
         self.config.update(json.loads(self.lib.pi05_config_json(self.handle).decode()))
         chain = self.config.get("chain")
@@ -181,6 +205,9 @@ class Pi05Arm:
         _lib.check(self.lib, self.handle, self.lib.pi05_refresh(self.handle))
 
     def launch(self) -> None:
+        if self.cached is not None:
+            cached, dense = self.cached
+            cached.cache.read(cached.table, self.geo.prefix, out=dense)
         stream = torch.cuda.current_stream(self.device).cuda_stream
         stamps = self.stamps.data_ptr() if self.stamps is not None else None
         _lib.check(self.lib, self.handle, self.lib.pi05_launch(self.handle, self.steps, self.layers, stream, stamps))
@@ -192,7 +219,7 @@ class Pi05Arm:
         if getattr(self, "handle", None):
             self.lib.pi05_destroy(self.handle)
             self.handle = None
-        self.tensors = None
+        self.tensors = self.cached = None
 
     def __del__(self) -> None:  # pragma: no cover
         try:

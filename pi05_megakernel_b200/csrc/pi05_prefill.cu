@@ -68,6 +68,21 @@ __global__ void __launch_bounds__(256) tables_kernel(const uint8_t* __restrict__
   }
 }
 
+// The same tables for tokens at given positions (a step behind a cached prefix).
+__global__ void __launch_bounds__(256) step_tables_kernel(const int* __restrict__ positions, int tokens, uint32_t* __restrict__ rope, unsigned int* status) {
+  __shared__ float s_inv[128];
+  const int tid = threadIdx.x, t0 = blockIdx.x * 32;
+  if (tid < 128) s_inv[tid] = 1.0f / (float)pow(10000.0, (double)((float)(2 * tid) / 256.0f));
+  if (blockIdx.x == 0 && tid < 2) status[tid] = 0u;
+  __syncthreads();
+  for (int i = tid; i < 32 * 128; i += 256) {
+    const int t = t0 + (i >> 7);
+    if (t >= tokens) break;
+    const float phase = (float)positions[t] * s_inv[i & 127];
+    rope[gemm::rope_at(tokens, t, i & 127)] = pack2((float)cos((double)phase), (float)sin((double)phase));
+  }
+}
+
 struct NormArgs {
   const __nv_bfloat16* src;        // the residual stream before this kernel
   __nv_bfloat16 *x, *out;          // the residual stream after it, and its norm
@@ -296,16 +311,21 @@ int pi05_prefill_bind(pi05_prefill_t h, const void* const weights[PI05_PREFILL_N
   return PI05_OK;
 }
 
-int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid, int tokens, void* keys, void* values,
-                     int n_layers, void* stream_) {
-  if (!h || !embeddings || !valid || !keys || !values) return PI05_ERR_ARGUMENT;
-  if (!h->bound) return PI05_ERR_NOT_BOUND;
-  if (tokens < 1 || tokens > h->max_tokens || n_layers < 1 || n_layers > pf::LAYERS) return PI05_ERR_ARGUMENT;
-  if ((reinterpret_cast<uintptr_t>(embeddings) & 15) || (reinterpret_cast<uintptr_t>(keys) & 15) ||
-      (reinterpret_cast<uintptr_t>(values) & 15)) {
-    h->last_error = "embeddings, keys and values must be 16-byte aligned";
-    return PI05_ERR_ARGUMENT;
-  }
+}  // extern "C"
+
+namespace {
+
+// What a step does in place of the prefill's attention: its keys and values go into the cache, and the queries attend to what lies there.
+struct Step {
+  const pi05_cache* cache;
+  pi05_shared_call call;              // without the queries and outputs
+  const int *positions, *starts;
+  void *hidden, *workspace;
+  size_t workspace_bytes;
+};
+
+// The layers over `tokens` rows, of a prefill (keys and values [layers][tokens][256] are its outputs) or of a step.
+int run_layers(pi05_prefill_t h, const void* embeddings, const void* valid, int tokens, void* keys, void* values, int n_layers, const Step* step, void* stream_) {
   Guard guard(h->device);
   if (!guard.ok) return PI05_ERR_CUDA;
   cudaStream_t stream = (cudaStream_t)stream_;
@@ -329,7 +349,7 @@ int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid
   if (part_floats(pl, P) > h->part_floats) { h->last_error = "the workspace does not hold the partial sums of this prompt"; return PI05_ERR_UNSUPPORTED; }
   for (const GemmPlan* g : {&pl.qkv, &pl.o, &pl.gu, &pl.down})
     if (e == cudaSuccess) e = opt_in_gemm(*g, h->device);
-  if (e == cudaSuccess) e = opt_in_attention(pl.tok_tile, false, h->device);
+  if (e == cudaSuccess && !step) e = opt_in_attention(pl.tok_tile, false, h->device);
   if (e != cudaSuccess) { h->last_error = cudaGetErrorString(e); return PI05_ERR_CUDA; }
 
   // tensor maps: activations (rows = tokens, zero beyond), weights (all layers stacked), keys / values for the attention
@@ -339,11 +359,11 @@ int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid
   const uint64_t L = pf::LAYERS;
   auto act_map = [&](CUtensorMap* m, const void* base, int k, const GemmPlan& g) { return map_k(m, base, k, P, g.arows, g.ks); };
   auto weight_map = [&](CUtensorMap* m, int which, int k, int rows, const GemmPlan& g) { return map_k(m, w[which], k, L * rows, g.w_rows, g.w_kb); };
-  const bool ok = act_map(&a_qkv, nrm, pf::H, pl.qkv) && act_map(&a_o, mixed, QD, pl.o) && act_map(&a_gu, nrm, pf::H, pl.gu) &&
+  bool ok = act_map(&a_qkv, nrm, pf::H, pl.qkv) && act_map(&a_o, mixed, QD, pl.o) && act_map(&a_gu, nrm, pf::H, pl.gu) &&
                   act_map(&a_dn, act, pf::FFN, pl.down) && weight_map(&wq, LQ, pf::H, QD, pl.qkv) && weight_map(&wk, LK, pf::H, HD, pl.qkv) &&
                   weight_map(&wv, LV, pf::H, HD, pl.qkv) && weight_map(&wo, LO, QD, pf::H, pl.o) && weight_map(&wg, LG, pf::H, pf::FFN, pl.gu) &&
-                  weight_map(&wu, LU, pf::H, pf::FFN, pl.gu) && weight_map(&wd, LD, pf::FFN, pf::H, pl.down) &&
-                  map_kv(&ap.pk, K, P, L, 1, HD, (uint64_t)P * HD, L * P * HD, attn::KCH, 2) &&
+                  weight_map(&wu, LU, pf::H, pf::FFN, pl.gu) && weight_map(&wd, LD, pf::FFN, pf::H, pl.down);
+  if (!step) ok = ok && map_kv(&ap.pk, K, P, L, 1, HD, (uint64_t)P * HD, L * P * HD, attn::KCH, 2) &&
                   map_kv(&ap.pv, V, P, L, 1, HD, (uint64_t)P * HD, L * P * HD, 64, 4) &&
                   map_k(&ap.q, q, HD, (uint64_t)P * NQH, pl.tok_tile * NQH, HD / 64);
   if (!ok) { h->last_error = "cuTensorMapEncodeTiled failed"; return PI05_ERR_CUDA; }
@@ -362,7 +382,7 @@ int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid
     if (b1) p.b1 = *b1;
     if (b2) p.b2 = *b2;
     p.tokens = P; p.layer = layer; p.width = width; p.unit0 = unit0; p.status = status; p.limit = h->wait_limit;
-    p.q = q; p.k = K + (size_t)layer * P * HD; p.v = V + (size_t)layer * P * HD; p.rope = rope; p.act = act; p.part = part;
+    p.q = q; p.k = step ? K : K + (size_t)layer * P * HD; p.v = step ? V : V + (size_t)layer * P * HD; p.rope = rope; p.act = act; p.part = part;
     e = launch_gemm(g, p, stream);
   };
   pf::NormArgs n;
@@ -381,26 +401,89 @@ int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid
     if (e == cudaSuccess) e = launch_chained(kernel, P, 512, 0, stream, 1, n);
   };
 
-  pf::tables_kernel<<<(P + 31) / 32, 256, 0, stream>>>(static_cast<const uint8_t*>(valid), P, rope, status);
+  int rc = PI05_OK;
+  auto attend = [&](int layer) {              // of a step
+    const pi05_cache_rows rows = {K, V, (long long)step->call.tokens * HD, 0, HD, 0, step->call.table, step->starts, nullptr, step->call.batch, 1,
+                                  step->call.tokens, layer, step->call.table_stride, step->call.table_pages};
+    pi05_shared_call call = step->call;
+    call.q = q; call.out = mixed; call.lse = nullptr; call.layer = layer; call.q_heads = NQH; call.scale = 0.0625f;
+    call.q_batch_stride = call.out_batch_stride = (long long)call.tokens * QD;
+    call.q_token_stride = call.out_token_stride = QD;
+    call.q_head_stride = call.out_head_stride = HD;
+    rc = pi05_cache_write(h->device, step->cache, &rows, stream);
+    if (rc == PI05_OK) rc = pi05_shared_attention(h->device, step->cache, &call, step->workspace, step->workspace_bytes, stream);
+    return rc == PI05_OK;
+  };
+
+  if (step) pf::step_tables_kernel<<<(P + 31) / 32, 256, 0, stream>>>(step->positions, P, rope, status);
+  else pf::tables_kernel<<<(P + 31) / 32, 256, 0, stream>>>(static_cast<const uint8_t*>(valid), P, rope, status);
   e = cudaGetLastError();
   norm(pf::norm_kernel<0>, static_cast<const __nv_bfloat16*>(embeddings), w[LN1]);
   for (int l = 0; l < n_layers && e == cudaSuccess; ++l) {
-    if (l + 1 == n_layers) {                      // keys and values only: the tiles behind the eight query heads
+    const bool last = l + 1 == n_layers;
+    if (last && !step) {                          // keys and values only: the tiles behind the eight query heads
       project(pl.qkv, a_qkv, wq, &wk, &wv, 0, l, pl.qkv.units / (NQH + 2) * NQH);
       break;
     }
     project(pl.qkv, a_qkv, wq, &wk, &wv, 0, l);
-    ap.layer = l;
-    if (e == cudaSuccess) e = launch_attention(ap, 1, stream);
+    if (step) {
+      if (e == cudaSuccess && !attend(l)) break;
+    } else {
+      ap.layer = l;
+      if (e == cudaSuccess) e = launch_attention(ap, 1, stream);
+    }
     project(pl.o, a_o, wo, nullptr, nullptr, pf::H, l);
     norm(pf::norm_kernel_for(pl.o.splits), x, w[LN2] + (size_t)l * pf::H);
     project(pl.gu, a_gu, wg, &wu, nullptr, pf::FFN, l);
     project(pl.down, a_dn, wd, nullptr, nullptr, pf::H, l);
-    norm(pl.sk_down ? (P <= h->sms ? pf::norm_kernel<-2> : pf::norm_kernel<-1>) : pf::norm_kernel_for(pl.down.splits), x, w[LN1] + (size_t)(l + 1) * pf::H);
+    if (last) n.x = static_cast<__nv_bfloat16*>(step->hidden);      // (its norm has no reader, nor a weight of its own)
+    norm(pl.sk_down ? (P <= h->sms ? pf::norm_kernel<-2> : pf::norm_kernel<-1>) : pf::norm_kernel_for(pl.down.splits), x, w[LN1] + (size_t)(last ? l : l + 1) * pf::H);
   }
+  if (rc != PI05_OK) { h->last_error = "the cache or the attention over it refused its arguments"; return rc; }
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) { h->last_error = std::string("kernel launch: ") + cudaGetErrorString(e); return PI05_ERR_CUDA; }
   return PI05_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pi05_prefill_run(pi05_prefill_t h, const void* embeddings, const void* valid, int tokens, void* keys, void* values,
+                     int n_layers, void* stream) {
+  if (!h || !embeddings || !valid || !keys || !values) return PI05_ERR_ARGUMENT;
+  if (!h->bound) return PI05_ERR_NOT_BOUND;
+  if (tokens < 1 || tokens > h->max_tokens || n_layers < 1 || n_layers > pf::LAYERS) return PI05_ERR_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(embeddings) & 15) || (reinterpret_cast<uintptr_t>(keys) & 15) ||
+      (reinterpret_cast<uintptr_t>(values) & 15)) {
+    h->last_error = "embeddings, keys and values must be 16-byte aligned";
+    return PI05_ERR_ARGUMENT;
+  }
+  return run_layers(h, embeddings, valid, tokens, keys, values, n_layers, nullptr, stream);
+}
+
+int pi05_prefill_step(pi05_prefill_t h, const pi05_cache* cache, const pi05_shared_call* call, const void* embeddings, const int* positions, const int* starts,
+                      void* hidden, int n_layers, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!h || !cache || !call || !embeddings || !positions || !starts || !hidden || !workspace) return PI05_ERR_ARGUMENT;
+  if (!h->bound) return PI05_ERR_NOT_BOUND;
+  const long long rows = (long long)call->batch * call->tokens;
+  if (call->batch < 1 || call->tokens < 1 || rows > h->max_tokens || n_layers < 1 || n_layers > pf::LAYERS || !call->table || !call->lengths ||
+      ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(starts)) & 3)) {
+    h->last_error = "a step needs tables, lengths, positions and starts, and at most as many tokens as the handle is made for";
+    return PI05_ERR_ARGUMENT;
+  }
+  if (((reinterpret_cast<uintptr_t>(embeddings) | reinterpret_cast<uintptr_t>(hidden)) & 15)) {
+    h->last_error = "embeddings and hidden must be 16-byte aligned";
+    return PI05_ERR_ARGUMENT;
+  }
+  if (cache->kv_heads != 1 || cache->head_dim != HD || cache->layers < n_layers) {
+    h->last_error = "the cache must hold the layers of Gemma-2B: one KV head of 256";
+    return PI05_ERR_UNSUPPORTED;
+  }
+  // the tokens' keys and values of a layer, until they are in the cache: where the MLP's activations go later
+  __nv_bfloat16* k = reinterpret_cast<__nv_bfloat16*>(h->ws + h->off_act);
+  const Step step = {cache, *call, positions, starts, hidden, workspace, workspace_bytes};
+  return run_layers(h, embeddings, nullptr, (int)rows, k, k + rows * HD, n_layers, &step, stream);
 }
 
 int pi05_prefill_plan(int sms, int tokens, int cta, int info[PI05_PREFILL_PLAN_INFO], int* segments, int capacity, int* count) {

@@ -1,4 +1,4 @@
-"""The Gemma-2B prefix prefill as a callable: the step before the action chunk.
+"""The Gemma-2B prefix prefill as a callable: the step before the action chunk, and steps of new tokens behind a cached prefix.
 
 Same call as the reference's ``prefill(case, values, embeddings, valid)`` (reference/pi05.py:167-195) without the case
 object: ``Pi05Prefill(geo, device)`` once, ``bind(values)`` with the nine BF16 weight tensors (kept by pointer, read in
@@ -14,7 +14,9 @@ import ctypes
 import torch
 
 from . import _lib
+from .cache import KvCache
 from .fixture import PREFILL_WEIGHTS, PrefillGeometry, prefill_shapes
+from .shared import CALL, SharedPrefixAttention
 
 
 class Pi05Prefill:
@@ -59,8 +61,12 @@ class Pi05Prefill:
         self.weights = tensors
 
     def run(self, embeddings: torch.Tensor, valid: torch.Tensor, layers: int | None = None,
-            out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """Asynchronous on the current stream.  ``embeddings`` [tokens, 2048] BF16, ``valid`` [tokens] bool."""
+            out: tuple[torch.Tensor, torch.Tensor] | None = None, cache: KvCache | None = None,
+            table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Asynchronous on the current stream.  ``embeddings`` [tokens, 2048] BF16, ``valid`` [tokens] bool.  With ``cache`` the keys and values also go
+        into the pages that ``table`` int32 [pages] names (``KvCache.write``)."""
+        if (cache is None) != (table is None):
+            raise ValueError("a cache needs the page table of the prompt, and a table its cache")
         tokens = embeddings.shape[0]
         if tuple(embeddings.shape) != (tokens, self.geo.hidden) or embeddings.dtype != torch.bfloat16 or \
                 tuple(valid.shape) != (tokens,) or valid.dtype != torch.bool:
@@ -76,7 +82,43 @@ class Pi05Prefill:
         stream = torch.cuda.current_stream(self.device).cuda_stream
         self._check(self.lib.pi05_prefill_run(self.handle, embeddings.data_ptr(), valid.data_ptr(), tokens, k.data_ptr(),
                                               v.data_ptr(), self.geo.layers if layers is None else layers, stream))
+        if cache is not None:
+            cache.write(k[None], v[None], table[None])
         return k, v
+
+    def step(self, embeddings: torch.Tensor, positions: torch.Tensor, attention: SharedPrefixAttention, prefix_table: torch.Tensor | None,
+             prefix_tokens: int, table: torch.Tensor, lengths: torch.Tensor, valid: torch.Tensor | None = None, causal: bool = True,
+             layers: int | None = None) -> torch.Tensor:
+        """New tokens of several sequences behind a prefix that they share, through the layers: ``embeddings`` BF16 ``[batch, tokens, 2048]`` at rotary
+        ``positions`` int32 ``[batch, tokens]``.  Per layer their keys and values go into ``attention.cache``, at the end of the sequences that
+        ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` (with these tokens) describe, and the queries attend to the prefix and to
+        their sequence; prefix, ``valid`` and ``causal`` as in ``SharedPrefixAttention.run``.  Returns the residual stream behind the last
+        layer, ``[batch, tokens, 2048]``; asynchronous on the current stream."""
+        if self.weights is None:
+            raise _lib.EngineError(_lib.ERR_NOT_BOUND, self.lib.pi05_error_string(_lib.ERR_NOT_BOUND).decode())
+        c = attention.cache
+        if embeddings.dim() != 3 or embeddings.shape[2] != self.geo.hidden or embeddings.dtype != torch.bfloat16 or positions.dtype != torch.int32 or \
+                positions.shape != embeddings.shape[:2]:
+            raise ValueError("embeddings must be [batch, tokens, 2048] bfloat16 and positions [batch, tokens] int32")
+        if not (embeddings.is_contiguous() and positions.is_contiguous()) or embeddings.device != self.device or positions.device != self.device or \
+                c.device != self.device:
+            raise ValueError(f"embeddings and positions must be contiguous and live on {self.device}, like the cache")
+        if attention.q_heads != self.geo.q_heads or c.kv_heads != 1 or c.head_dim != self.geo.head_dim:
+            raise ValueError("the attention must be one of 8 query heads over a cache of one KV head of 256")
+        if table is None or lengths is None:
+            raise ValueError("a step needs the sequences' tables and lengths")
+        batch, tokens = embeddings.shape[:2]
+        # the checks of an attention call; queries and outputs are the handle's own
+        like = torch.empty((batch, tokens, self.geo.q_heads, self.geo.head_dim), dtype=torch.bfloat16, device="meta")
+        fit = attention._fit(like, like, prefix_table, prefix_tokens, table, lengths, 0, valid, causal, None, shapes_only=True)
+        hidden = torch.empty_like(embeddings)
+        starts = lengths - tokens
+        call = CALL.pack(0, 0, 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0, valid.data_ptr() if prefix_tokens and valid is not None else 0,
+                         table.data_ptr(), lengths.data_ptr(), *fit[6:])
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        self._check(self.lib.pi05_prefill_step(self.handle, c.ref, call, embeddings.data_ptr(), positions.data_ptr(), starts.data_ptr(), hidden.data_ptr(),
+                                               self.geo.layers if layers is None else layers, attention.workspace, attention.nbytes, stream))
+        return hidden
 
     def status(self) -> None:
         """Synchronise the current stream; raises when a bounded device-side wait gave up."""

@@ -65,10 +65,10 @@ class SharedPrefixAttention:
             _lib.check(self.lib, None, rc)
         return (out, lse) if with_lse else out
 
-    def _fit(self, q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale):
+    def _fit(self, q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale, shapes_only=False):
         """What does not depend on addresses, checked, as in ``KvCache``."""
         c = self.cache
-        if q.dim() != 4 or q.dtype != torch.bfloat16 or q.device != self.device or q.shape[2] != self.q_heads or q.shape[3] != c.head_dim:
+        if q.dim() != 4 or q.dtype != torch.bfloat16 or (q.device != self.device and not shapes_only) or q.shape[2] != self.q_heads or q.shape[3] != c.head_dim:
             raise ValueError(f"q must be bfloat16 [batch, tokens, {self.q_heads}, {c.head_dim}] on {self.device}")
         batch, tokens = q.shape[:2]
         if batch > self.max_batch or tokens > self.max_tokens:
@@ -76,7 +76,7 @@ class SharedPrefixAttention:
         scale = c.head_dim ** -0.5 if scale is None else scale
         if not 0 <= layer < c.layers or prefix_tokens < 0 or not 0 < scale < float("inf"):
             raise ValueError("no such layer in the cache, a negative prefix_tokens, or a scale that is not positive and finite")
-        if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device:
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or (out.device != self.device and not shapes_only):
             raise ValueError("out must be like q")
         qs, os_ = strides(q), strides(out)
         if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_):

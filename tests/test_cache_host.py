@@ -74,6 +74,11 @@ def test_bad_calls_are_refused(lib, change):
     assert lib.pi05_shared_attention(-1, cache(), call(), 0x100000, 1 << 30, None) == _lib.ERR_ARGUMENT
 
 
+def test_bad_steps_are_refused(lib):
+    """Without a handle, and before anything is followed."""
+    assert lib.pi05_prefill_step(None, cache(), call(), 0x1000, 0x1000, 0x1000, 0x1000, 1, 0x100000, 1 << 30, None) == _lib.ERR_ARGUMENT
+
+
 def test_workspace(lib):
     """It grows with batch and tokens, holds any smaller call's, and a call refuses one that is too small, not aligned or missing."""
     n, last = ctypes.c_size_t(), 0
