@@ -30,6 +30,21 @@ def check_table(name: str, t: torch.Tensor, device: torch.device, dim: int) -> N
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+class Fresh:
+    """New tensors like those of earlier calls: from a template (one element, expanded) an allocation takes 1.3 us, from sizes, type and device 2.5 to 3.3."""
+
+    def __init__(self, device: torch.device) -> None:
+        self.device, self.templates = device, {}
+
+    def __call__(self, shape, dtype: torch.dtype) -> torch.Tensor:
+        t = self.templates.get((shape, dtype))
+        if t is None:
+            if len(self.templates) >= MAX_FITS:
+                self.templates.clear()
+            t = self.templates[(shape, dtype)] = torch.empty(1, dtype=dtype, device=self.device).expand(shape)
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def describe(t: torch.Tensor | None):
     """What a check of a table goes by."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
@@ -88,7 +103,7 @@ class KvCache:
         self.words = torch.zeros(4, dtype=torch.int32, device=self.device)       # the status words
         scale = (None, None) if k_scale is None else (k_scale.data_ptr(), v_scale.data_ptr())
         self.struct = _lib.Cache(k.data_ptr(), v.data_ptr(), *scale, self.words.data_ptr(), FORMATS[self.format][0], *k.shape)
-        self.ref, self.index, self.fits = ctypes.byref(self.struct), self.device.index, {}
+        self.ref, self.index, self.fits, self.fresh = ctypes.byref(self.struct), self.device.index, {}, Fresh(self.device)
         self.call_write, self.call_read = self.lib.pi05_cache_write, self.lib.pi05_cache_read
         # what the library refuses is refused here, before a first call
         nbytes = ctypes.c_size_t()
@@ -145,7 +160,7 @@ class KvCache:
             layers = self.layers - layer
         if out is None:
             shape = (table.shape[0], layers, tokens, self.kv_heads, self.head_dim)
-            out = (torch.empty(shape, dtype=torch.bfloat16, device=self.device), torch.empty(shape, dtype=torch.bfloat16, device=self.device))
+            out = (self.fresh(shape, torch.bfloat16), self.fresh(shape, torch.bfloat16))
         elif out[0].shape[1:3] != (layers, tokens):
             raise ValueError("out does not have the layers and tokens that are read")
         rc = self.call_read(self.index, self.ref, self._rows(*out, table, starts, counts, layer), raw_stream(self.index))

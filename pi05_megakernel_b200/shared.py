@@ -32,6 +32,7 @@ class SharedPrefixAttention:
         sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         _lib.check(self.lib, None, self.lib.pi05_shared_workspace(sms, cache.ref, q_heads, max_batch, max_tokens, ctypes.byref(nbytes)))
         self.ws = torch.zeros(nbytes.value, dtype=torch.uint8, device=self.device)
+        self.fresh = cache.fresh
         self.workspace, self.nbytes, self.index, self.fits, self.call = self.ws.data_ptr(), nbytes.value, self.device.index, {}, self.lib.pi05_shared_attention
 
     def run(self, q: torch.Tensor, prefix_table: torch.Tensor | None, prefix_tokens: int, table: torch.Tensor | None = None,
@@ -44,10 +45,10 @@ class SharedPrefixAttention:
         of them count (None: all).  ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` are the sequences' own tokens, the
         queries' among them; ``causal``: query t sees own tokens up to its own place, ``lengths[b] - tokens + t``, else all of them.
         ``scale`` defaults to head_dim ** -0.5.  A query that sees no key gets zeros (log-sum-exp: -infinity)."""
+        key = (q.shape, q.stride(), q.dtype, q.device, describe(out), describe(prefix_table), prefix_tokens, describe(table), describe(lengths),
+               describe(valid), layer, causal, scale)
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-        key = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device, describe(prefix_table), prefix_tokens, describe(table),
-               describe(lengths), describe(valid), layer, causal, scale)
+            out = self.fresh(q.shape, torch.bfloat16)
         fit = self.fits.get(key)
         if fit is None:
             if len(self.fits) >= MAX_FITS:
@@ -56,7 +57,7 @@ class SharedPrefixAttention:
         qp, op = q.data_ptr(), out.data_ptr()
         if (qp | op) & 15:
             raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=self.device) if with_lse else None
+        lse = self.fresh(q.shape[:3], torch.float32) if with_lse else None
         call = CALL.pack(qp, op, lse.data_ptr() if with_lse else 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0,
                          valid.data_ptr() if prefix_tokens and valid is not None else 0, 0 if table is None else table.data_ptr(),
                          0 if lengths is None else lengths.data_ptr(), *fit[6:])
