@@ -362,7 +362,9 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
 /* Attention of batch x tokens queries over one prefix that all sequences share and over each sequence's own tokens:
  *   out = sum_j p_j v_j,  p = softmax(scale q . k_j)  over the prefix tokens j < prefix_tokens with prefix_valid[j] != 0 (NULL: all) and the own
  * tokens j < lengths[b] of sequence b; causal: own tokens j <= lengths[b] - tokens + t for query t, so that the queries are the last tokens
- * of the sequence.  What masked places of the cache hold does not matter.  A query without any key gets zeros and lse -infinity.
+ * of the sequence.  What places of the cache hold that a query does not see does not matter to it; one that sees an infinity or a NaN gets outputs that
+ * are not finite (all of its outputs are NaN where other queries of the sequence do not see it).  A query without any key gets zeros and lse -infinity.
+ * At most 1024 sequences and 2^27 query rows (batch x tokens x q_heads) a call.
  * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8; query head h uses KV head
  * h / (q_heads / kv_heads).  lse (NULL: not wanted): [batch][tokens][q_heads] FP32, the logarithm of the sum of exp(scale q . k_j).
  * table = NULL: no own tokens.  Scores, softmax and sums are FP32; probabilities are rounded to BF16 (times the value's scale, 8 bits)

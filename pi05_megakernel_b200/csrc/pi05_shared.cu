@@ -87,7 +87,6 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   a.c = c; a.s = s;
   a.group = s.q_heads / c.kv_heads;
   a.piece = c.page_tokens % 64 == 0 ? 64 : c.page_tokens % 32 == 0 ? 32 : 16;
-  a.whole = a.piece == 64;
   a.a_tiles = (int)k.a_tiles; a.b_tiles = (int)k.b_tiles; a.b_rows = (int)k.b_rows; a.b_slot = (int)k.b_slot;
   a.overhead = shared::overhead(c.format);
   a.p_tiles = (s.prefix_tokens + shared::TILE - 1) / shared::TILE;

@@ -55,7 +55,6 @@ struct Args {
   pi05_cache c;
   pi05_shared_call s;
   int piece;                                // tokens of a copy: 64, 32 or 16, which divides the page
-  int whole;                                // BF16: a copy brings all head_dim elements (pieces of 64 tokens), else 64 of them
   int group;                                // query heads per KV head
   int joined;
   int a_tiles;                              // row tiles of the batch against the prefix (not joined)
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   constexpr int TM_O = 0, TM_Q = DIM, TM_S = TM_Q + Q_BUFS * DIM / 2, TM_P = OVER ? TM_S : TM_S + S_BUFS * TILE, P_STEP = OVER ? TILE : TILE / 2;
   static_assert(TM_P + 2 * P_STEP <= 512, "tensor memory");
   constexpr int TM_COLS = 512;
-  constexpr int TOKEN = 1, END = 9;         // named barriers of a pair of softmax warps: reference handed on (by group), end of a segment
+  constexpr int TOKEN = 1, END = 9, LOST = 13;      // named barriers: of a pair of softmax warps, reference handed on (by group), end of a segment; of a group
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[4 * INFO + 2 * UNITS + 2 * RAW + Q_BUFS + 2 * S_BUFS + 5];
@@ -307,6 +306,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   __shared__ float2 s_ml[2][2][ROWS];       // at its end: the groups' references and sums
   __shared__ Segment s_seg[threads(FORMAT) / 32], s_ahead[8];      // a warp's segment; a softmax warp's next one
   __shared__ Walk s_walk;
+  __shared__ uint32_t s_lost[2][2][2];      // by group and turn: keys of a ragged tile whose values are not all numbers
   __shared__ __align__(16) float s_ones[CODES ? TILE : 1];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
 #define WAIT_ONE(BAR, PARITY, KIND) wait_one(p, BAR, PARITY, KIND)
 
   if (CODES && tid < TILE) s_ones[tid] = 1.f;
+  if (!CODES && tid < 8) (&s_lost[0][0][0])[tid] = 0u;
   if (warp == 0) {
     auto init = [&](uint32_t b, int n, int count) { for (int i = lane; i < n; i += 32) ptx::mbar_init(b + 8 * i, count); };
     init(info_full, INFO, 1); init(info_empty, INFO, CODES ? 6 : 5); init(scale_full, INFO, 1); init(vlog_full, INFO, 1);
@@ -635,6 +636,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
       const int count = d.n;
       int own;                              // of the segment's first tile: its place among the tiles of own tokens
       int sees;                             // own tokens that the row sees
+      int all_see;                          // and those that all rows of the item do
       bool mine, idle;
       {
         int b = 0, t = 0, head = 0;
@@ -643,6 +645,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         own = d.first - (d.batch || p.joined ? p.p_tiles : 0);
         const int length = d.batch ? 0 : lengths[d.b];
         sees = p.s.causal ? length - p.s.tokens + t + 1 : length;
+        all_see = p.s.causal && p.s.tokens > 1 ? length - p.s.tokens + 1 : 0x7fffffff;
       }
       float m = -INFINITY, l = 0.f;         // reference (of exponents to the base 2) and sum
       at = next_segment(p, walk, at, &ahead);
@@ -786,17 +789,35 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           if (poison) l = __uint_as_float(0x7fffffffu);
           ptx::tmem_wait_st();
         }
-        if (!CODES && (mask0 & mask1 & ~(bad0 | bad1)) != 0xffffffffu) {
-          // values at places that do not count are whatever memory holds, and 0 x NaN is NaN: zeros in their place
-          const uint32_t u = unit + v_unit(i, count), at = u % UNITS;
+        // Values at places that do not count are whatever memory holds, and 0 x NaN is NaN: zeros in their place.  Where only some of the tile's rows see a token
+        // (`ragged`) the same for an infinity or a NaN among its values, and the rows that do see it get NaN
+        const bool ragged = !CODES && own + i >= 0 && (own + i + 1) * TILE > all_see;
+        if (!CODES && (ragged || (mask0 & mask1 & ~(bad0 | bad1)) != 0xffffffffu)) {
+          const uint32_t u = unit + v_unit(i, count), at = u % UNITS, turn = n >> 1 & 1;
           ok = ok && WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
           const uint32_t z0 = ~mask0 | bad0, z1 = ~mask1 | bad1;
+          if (ragged && row < 2) s_lost[group][turn ^ 1][row] = 0u;        // (the group's last tile but one: everybody is through with it)
+#pragma unroll 1
           for (int c = row; c < TILE * DIM / 8; c += 128) {
             const int key = c & 63, chunk = c >> 6;
-            if ((key < 32 ? z0 : z1) >> (key & 31) & 1) ptx::st_shared_v4(ring + at * UNIT + (chunk >> 3) * (TILE * 128) + key * 128 + (chunk & 7) * 16, 0u, 0u, 0u, 0u);
+            const uint32_t line = ring + at * UNIT + (chunk >> 3) * (TILE * 128) + key * 128 + (chunk & 7) * 16;
+            bool clear = (key < 32 ? z0 : z1) >> (key & 31) & 1;
+            if (ragged && !clear) {
+              const uint4 x = ptx::ld_shared_v4(line);
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) clear |= (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+              if (clear) atomicOr(&s_lost[group][turn][key >> 5], 1u << (key & 31));
+            }
+            if (clear) ptx::st_shared_v4(line, 0u, 0u, 0u, 0u);
           }
           ptx::fence_proxy_async_shared();
+          if (ragged) {
+            ptx::named_bar_sync(LOST + group, 128);
+            if ((k0 & s_lost[group][turn][0]) | (k1 & s_lost[group][turn][1])) l = __uint_as_float(0x7fffffffu);
+          }
         }
+        __syncwarp();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) {

@@ -242,6 +242,33 @@ def test_a_key_that_is_not_a_number():
     assert bool(torch.isfinite(got[0]).all()) and bool(torch.isfinite(got[1, :2]).all()) and bool(torch.isnan(got[1, 2:]).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_numbers_stay_with_those_that_see_them(dim, bad):
+    """BF16: keys and values that are not numbers, at tokens that only some of a sequence's queries see, reach those and nobody else, whichever group of
+    warps has the tile."""
+    from pi05_megakernel_b200.shared import SharedPrefixAttention
+    tokens, q_heads = 70, 3
+    c, ptab, tab, lengths, rnd = build("bf16", 2, 100, 300, 16, 1, dim, junk=False)
+    lengths.copy_(torch.tensor([300, 250]))
+    q = rnd(2, tokens, q_heads, dim)
+    op = SharedPrefixAttention(c, q_heads, 2, tokens)
+    clean = op.run(q, ptab, 100, tab, lengths, layer=1)
+    for token in (299, 290, 256, 255, 232):                               # of sequence 0, whose queries stand at 230 .. 299
+        for pool in (c.k, c.v):
+            page, at = int(tab[0, token // 16]), token % 16
+            old = pool[page, 1, at].clone()
+            pool[page, 1, at, 0, dim - 3] = bad
+            got = op.run(q, ptab, 100, tab, lengths, layer=1)
+            op.status()
+            first = token - 230                                           # the first query that sees it
+            assert torch.equal(got[1], clean[1]) and torch.equal(got[0, :first], clean[0, :first])
+            if pool is c.v or bad != bad:
+                assert not bool(torch.isfinite(got[0, first:]).all(-1).any())
+            pool[page, 1, at] = old
+    assert torch.equal(op.run(q, ptab, 100, tab, lengths, layer=1), clean)
+
+
 def test_python_refusals():
     from pi05_megakernel_b200.shared import SharedPrefixAttention
     c, ptab, tab, lengths, rnd = build("int8", 2, 40, 20, 16, 2, 64)
