@@ -795,21 +795,31 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         if (!CODES && (ragged || (mask0 & mask1 & ~(bad0 | bad1)) != 0xffffffffu)) {
           const uint32_t u = unit + v_unit(i, count), at = u % UNITS, turn = n >> 1 & 1;
           ok = ok && WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
-          const uint32_t z0 = ~mask0 | bad0, z1 = ~mask1 | bad1;
-          if (ragged && row < 2) s_lost[group][turn ^ 1][row] = 0u;        // (the group's last tile but one: everybody is through with it)
+          const uint32_t z0 = ~mask0 | bad0, z1 = ~mask1 | bad1, line = ring + at * UNIT;
+          // a key's row by D / 8 lanes, sixteen keys a warp
+          const uint32_t mine_clear = (quad & 2 ? z1 : z0) >> (16 * (quad & 1));
+#pragma unroll 4
+          for (int c = lane / (DIM / 8); c < 16; c += 32 / (DIM / 8))
+            if (mine_clear >> c & 1)
+              ptx::st_shared_v4(line + (lane % (DIM / 8) >> 3) * (TILE * 128) + (16 * quad + c) * 128 + (lane & 7) * 16, 0u, 0u, 0u, 0u);
+          if (ragged) {
+            if (row < 2) s_lost[group][turn ^ 1][row] = 0u;                // (the group's last tile but one: everybody is through with it)
 #pragma unroll 1
-          for (int c = row; c < TILE * DIM / 8; c += 128) {
-            const int key = c & 63, chunk = c >> 6;
-            const uint32_t line = ring + at * UNIT + (chunk >> 3) * (TILE * 128) + key * 128 + (chunk & 7) * 16;
-            bool clear = (key < 32 ? z0 : z1) >> (key & 31) & 1;
-            if (ragged && !clear) {
-              const uint4 x = ptx::ld_shared_v4(line);
+            for (int c = row; c < TILE * DIM / 8; c += 128) {
+              const int key = c & 63, chunk = c >> 6;
+              const uint32_t to = line + (chunk >> 3) * (TILE * 128) + key * 128 + (chunk & 7) * 16;
+              if ((key < 32 ? z0 : z1) >> (key & 31) & 1) continue;
+              const uint4 x = ptx::ld_shared_v4(to);
               const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              bool found = false;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) clear |= (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
-              if (clear) atomicOr(&s_lost[group][turn][key >> 5], 1u << (key & 31));
+              for (int k = 0; k < 4; ++k) found |= (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+              if (found) {
+                atomicOr(&s_lost[group][turn][key >> 5], 1u << (key & 31));
+                ptx::st_shared_v4(to, 0u, 0u, 0u, 0u);
+              }
             }
-            if (clear) ptx::st_shared_v4(line, 0u, 0u, 0u, 0u);
+            __syncwarp();
           }
           ptx::fence_proxy_async_shared();
           if (ragged) {
