@@ -4,7 +4,7 @@
 //
 //   * Query rows of one KV head are packed into tiles of 128: of the whole batch against the prefix, so that its keys and values are read
 //     once for 128 / (tokens x group) sequences, of one sequence against its own tokens.  Where a sequence fills its tiles by itself (`joined`)
-//     prefix and own tokens are one list of keys and nothing has to be put together afterwards.
+//     prefix and own tokens are one list of keys.
 //   * Q, P, S and O all live in tensor memory (D = 256: 128 + 2 x 64 + 256 columns, P in place of S): both products take their A operand from
 //     there, an MMA only reads its 64 keys or head_dim values from shared memory, and all of it is a ring of keys and values: what this
 //     kernel mostly is bound by are the bytes of the cache.
@@ -18,7 +18,12 @@
 //   * Of an 8-bit cache two more groups turn codes into 16 bits, exactly: keys into BF16, as the queries are, values into FP16.  A key's scale
 //     multiplies its score and a value's scale its probability, both in FP32.  The product, rounded to FP16, keeps four bits more than
 //     BF16 would; so that it stays in FP16's range whatever the scales are, the reference of a row takes in the largest scale of
-//     the tile (warp 3 finds it): a shift that the division by the row's sum takes out again.
+//     the tile (warp 3 finds it): a shift that the division by the row's sum takes out again.  (In BF16 the outputs were 0.0025 off the definition, relative to
+//     0.0017 of their own rounding; now 0.0017.)
+//
+// What bounds it (one B200, both kernels): 64 sequences over 16384 tokens in BF16 78 us beside 31 of HBM, 224 MB read at 2.9 TB/s, tensor pipe 24%: the chain of a tile
+// through one group (2800 cycles for 64 keys) and the latency of 512 short items; drafts in e4m3 121 us beside 21 of tensor pipe: instructions of softmax and
+// converters; steps of a few sequences 12 to 18 us: launch, lengths, page lookup, first bytes, one tile, its parts and the second kernel, one after the other.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -295,6 +300,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   constexpr int TM_O = 0, TM_Q = DIM, TM_S = TM_Q + Q_BUFS * DIM / 2, TM_P = OVER ? TM_S : TM_S + S_BUFS * TILE, P_STEP = OVER ? TILE : TILE / 2;
   static_assert(TM_P + 2 * P_STEP <= 512, "tensor memory");
   constexpr int TM_COLS = 512;
+  constexpr int CHUNK = CODES ? 16 : 32;    // scores that a softmax thread takes at a time: the code of an 8-bit cache's warps is the longer one
   constexpr int TOKEN = 1, END = 9, LOST = 13;      // named barriers: of a pair of softmax warps, reference handed on (by group), end of a segment; of a group
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -674,32 +680,38 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         ptx::tc_fence_after();
         const float4* ks = reinterpret_cast<const float4*>(s_scales + slot * 2 * TILE);
         const uint32_t s_at = lanes + TM_S + sbuf * TILE, p_at = lanes + TM_P + buf * P_STEP;
-        // A tile is read twice, 32 scores at a time: for the row's maximum, then for the probabilities.  (With all 64 in registers
-        // the kernel's code is twice as long, and what its warps execute no longer fits the instruction cache)
+        // A tile is read twice, CHUNK scores at a time: for the row's maximum, then for the probabilities.  (What the warps of a CTA execute per tile has to fit the
+        // instruction cache.  With all 64 scores in registers 26% of the fetches missed it and drafts, 32 x 8 over 8192 in e4m3, took 245 us; read
+        // twice in 32s 14%, 142; in 16s and with the converters' loop rolled 121)
+        auto load_chunk = [](uint32_t from, float (&x)[CHUNK]) {
+          if constexpr (CHUNK == 32) ptx::tmem_ld_32x32(from, reinterpret_cast<uint32_t(&)[32]>(x));
+          else ptx::tmem_ld_32x16(from, reinterpret_cast<uint32_t(&)[16]>(x));
+          ptx::tmem_wait_ld();
+        };
         float high = -INFINITY;
         if (!idle) {
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            float x[32];
-            ptx::tmem_ld_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
-            ptx::tmem_wait_ld();
+          for (int h = 0; h < TILE; h += CHUNK) {
+            float x[CHUNK];
+            load_chunk(s_at + h, x);
             if (CODES) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 f = ks[h * 8 + j / 4];
+              for (int j = 0; j < CHUNK; j += 4) {
+                const float4 f = ks[(h + j) / 4];
                 const float2 y = mul2(make_float2(x[j], x[j + 1]), make_float2(f.x, f.y)), z = mul2(make_float2(x[j + 2], x[j + 3]), make_float2(f.z, f.w));
                 x[j] = y.x; x[j + 1] = y.y; x[j + 2] = z.x; x[j + 3] = z.y;
               }
             }
             if (special) {                  // keys that do not count: -infinity, there (scaled) for the second time too
-              const uint32_t k = h ? k1 : k0;
+              const uint32_t k = (h < 32 ? k0 : k1) >> (h & 31);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = k >> j & 1 ? x[j] : -INFINITY;
-              tmem_st_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
+              for (int j = 0; j < CHUNK; ++j) x[j] = k >> j & 1 ? x[j] : -INFINITY;
+#pragma unroll
+              for (int j = 0; j < CHUNK; j += 8) ptx::tmem_st_32x8(s_at + h + j, reinterpret_cast<uint32_t(&)[8]>(x[j]));
             }
             float a = high, b = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
+            for (int j = 0; j < CHUNK; j += 4) {
               a = fmaxf(fmaxf(a, x[j]), x[j + 1]);
               b = fmaxf(fmaxf(b, x[j + 2]), x[j + 3]);
             }
@@ -752,16 +764,15 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float4* scale = special ? reinterpret_cast<const float4*>(s_ones) : ks;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            float x[32];
-            ptx::tmem_ld_32x32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(x));
-            ptx::tmem_wait_ld();
-            uint32_t pk[16];
+          for (int h = 0; h < TILE; h += CHUNK) {
+            float x[CHUNK];
+            load_chunk(s_at + h, x);
+            uint32_t pk[CHUNK / 2];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
+            for (int j = 0; j < CHUNK; j += 4) {
               float2 e = make_float2(x[j], x[j + 1]), f = make_float2(x[j + 2], x[j + 3]);
               if (CODES) {
-                const float4 s = scale[h * 8 + j / 4];
+                const float4 s = scale[(h + j) / 4];
                 e = mul2(e, make_float2(s.x, s.y));
                 f = mul2(f, make_float2(s.z, s.w));
               }
@@ -771,7 +782,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
               sum[0] = add2(sum[0], e);
               sum[1] = add2(sum[1], f);
               if (CODES) {
-                const float4 s = ks[TILE / 4 + h * 8 + j / 4];
+                const float4 s = ks[(TILE + h + j) / 4];
                 e = mul2(e, make_float2(s.x, s.y));
                 f = mul2(f, make_float2(s.z, s.w));
                 asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[j / 2]) : "f"(e.y), "f"(e.x));
@@ -781,8 +792,8 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
                 pk[j / 2 + 1] = cache::pack2(f.x, f.y);
               }
             }
-            ptx::tmem_st_32x8(p_at + 16 * h, reinterpret_cast<uint32_t(&)[8]>(pk[0]));
-            ptx::tmem_st_32x8(p_at + 16 * h + 8, reinterpret_cast<uint32_t(&)[8]>(pk[8]));
+#pragma unroll
+            for (int j = 0; j < CHUNK / 2; j += 8) ptx::tmem_st_32x8(p_at + h / 2 + j, reinterpret_cast<uint32_t(&)[8]>(pk[j]));
           }
           const float2 both = add2(sum[0], sum[1]);
           l += both.x + both.y;
@@ -914,7 +925,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         if (!ok) break;
         constexpr int TURNS = TILE / ROWS_AT_ONCE / 4;
         auto turns = [&](auto value) {
-#pragma unroll 2
+#pragma unroll 1                        // (unrolled twice, drafts of 121 us took 142: the instruction cache)
           for (int j = 0; j < TURNS; ++j) {
             const int r = (j * 4 + w) * ROWS_AT_ONCE + first;
             const uint4 x = ptx::ld_shared_v4(raw + from * RAW_UNIT + r * DIM + blk * 64 + chunk * 16);
@@ -946,7 +957,8 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
 }
 
 // The unfinished items of a launch put together.  A warp has eight query rows x 16 dims (a line of every 16 bytes of a part), of which `split` warps of a
-// block take every split-th part each, eight at a time: what bounds it is how many loads are on their way.
+// block take every split-th part each, eight at a time: what bounds it is how many loads are on their way (with four at a time and no more than eight warps a row 13
+// queries over 30001 tokens, 148 parts, took 36.4 us, now 32).
 constexpr int COMBINE_THREADS = 512, AT_ONCE = 8;
 template <int DIM>
 __global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const __grid_constant__ Args p, int split) {
