@@ -364,7 +364,8 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
  * tokens j < lengths[b] of sequence b; causal: own tokens j <= lengths[b] - tokens + t for query t, so that the queries are the last tokens
  * of the sequence.  What places of the cache hold that a query does not see does not matter to it; one that sees an infinity or a NaN gets outputs that
  * are not finite (all of its outputs are NaN where other queries of the sequence do not see it).  A query without any key gets zeros and lse -infinity.
- * At most 1024 sequences and 2^27 query rows (batch x tokens x q_heads) a call.
+ * At most 1024 sequences and 2^27 query rows (batch x tokens x q_heads) a call.  A prefix, and a row of the table, reaches
+ * over at most 2^30 tokens.
  * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8; query head h uses KV head
  * h / (q_heads / kv_heads).  lse (NULL: not wanted): [batch][tokens][q_heads] FP32, the logarithm of the sum of exp(scale q . k_j).
  * table = NULL: no own tokens.  Scores, softmax and sums are FP32; probabilities are rounded to BF16 (times the value's scale, 8 bits)

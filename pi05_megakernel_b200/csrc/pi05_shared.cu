@@ -76,6 +76,8 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
       (((uintptr_t)s.lse | (uintptr_t)s.prefix_table | (uintptr_t)s.table | (uintptr_t)s.lengths) & 3) || !(s.scale > 0.f && s.scale < INFINITY))
     return PI05_ERR_ARGUMENT;
   if (s.batch > shared::MAX_BATCH || (long long)s.batch * s.tokens * s.q_heads > 1ll << 27) return PI05_ERR_UNSUPPORTED;
+  // places of keys are counted in 32 bits, in whole tiles: far enough from their end that rounding up does not pass it
+  if (s.prefix_tokens > 1 << 30 || (s.table && (long long)s.table_pages * c.page_tokens > 1ll << 30)) return PI05_ERR_UNSUPPORTED;
   DeviceGuard guard(device);
   int sms = 0;
   if (!guard.ok || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }

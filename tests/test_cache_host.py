@@ -136,3 +136,9 @@ def test_packed_arguments_are_the_structures():
 
 def test_error_string_of_a_page_table(lib):
     assert b"page" in lib.pi05_error_string(_lib.ERR_PAGE_TABLE)
+
+
+def test_places_of_keys_stay_in_32_bits(lib):
+    """A prefix or a table of more than 2^30 tokens, whose whole tiles would pass the end of an int, is refused before a device is asked for."""
+    for change in (dict(prefix_tokens=(1 << 30) + 1), dict(prefix_tokens=(1 << 31) - 1), dict(table_pages=(1 << 24) + 1), dict(table_pages=(1 << 31) - 1)):
+        assert lib.pi05_shared_attention(0, cache(), call(**change), 0x100000, 1 << 40, None) == _lib.ERR_UNSUPPORTED
