@@ -163,6 +163,8 @@ class KvCache:
             out = (self.fresh(shape, torch.bfloat16), self.fresh(shape, torch.bfloat16))
         elif out[0].shape[1:3] != (layers, tokens):
             raise ValueError("out does not have the layers and tokens that are read")
+        elif any(s == 0 and n > 1 for n, s in zip(out[0].shape, out[0].stride())):
+            raise ValueError("the rows of out must lie in different places")
         rc = self.call_read(self.index, self.ref, self._rows(*out, table, starts, counts, layer), raw_stream(self.index))
         if rc:
             _lib.check(self.lib, None, rc)

@@ -39,7 +39,7 @@ class SharedPrefixAttention:
             lengths: torch.Tensor | None = None, layer: int = 0, valid: torch.Tensor | None = None, causal: bool = True,
             scale: float | None = None, out: torch.Tensor | None = None, with_lse: bool = False):
         """Asynchronous on the current stream.  ``q`` BF16 ``[batch, tokens, q_heads, head_dim]`` of any strides; returns the outputs in the same
-        shape and, ``with_lse``, their log-sum-exp FP32 ``[batch, tokens, q_heads]``.
+        shape (in ``out``, whose rows lie in different places and not over ``q``) and, ``with_lse``, their log-sum-exp FP32 ``[batch, tokens, q_heads]``.
 
         ``prefix_table`` int32 ``[pages]`` names the pages of the ``prefix_tokens`` shared tokens, ``valid`` bool ``[prefix_tokens]`` which
         of them count (None: all).  ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` are the sequences' own tokens, the
@@ -82,6 +82,8 @@ class SharedPrefixAttention:
         qs, os_ = strides(q), strides(out)
         if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_):
             raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
+        if any(s == 0 and n > 1 for n, s in zip(out.shape, os_)):
+            raise ValueError("the rows of out must lie in different places")
         if prefix_tokens:
             if prefix_table is None:
                 raise ValueError("a prefix needs its page table")

@@ -277,3 +277,14 @@ def test_many_rows_behind_32_bits_of_elements():
     want = codes * scale[..., None]
     assert bool(((got.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all())
     assert int(c.k[-1, 0, :page - 40].count_nonzero()) == 0 and int(c.k[:-1].view(torch.int64).count_nonzero()) == 0
+
+
+def test_expanded_outputs_are_refused():
+    c = make("int8", 4, 2, 16, 2, 64)
+    t = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    one = torch.zeros(1, 2, 8, 2, 64, dtype=torch.bfloat16, device="cuda").expand(2, -1, -1, -1, -1)
+    with pytest.raises(ValueError):
+        c.read(t, 8, out=(one, one.clone().expand_as(one)))
+    with pytest.raises(ValueError):
+        c.read(t, 8, out=(one, one))
+    c.status()

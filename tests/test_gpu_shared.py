@@ -336,3 +336,15 @@ def test_two_calls_at_once():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     c.status()
+
+
+def test_expanded_outputs_are_refused():
+    from pi05_megakernel_b200.shared import SharedPrefixAttention
+    c, ptab, tab, lengths, rnd = build("bf16", 2, 40, 20, 16, 2, 64)
+    op, q = SharedPrefixAttention(c, 4, 2, 2), rnd(2, 2, 4, 64)
+    for out in (q[:1].clone().expand(2, -1, -1, -1), q[:, :1].clone().expand(-1, 2, -1, -1)):
+        with pytest.raises(ValueError):
+            op.run(q, ptab, 40, tab, lengths, out=out)
+    # queries may be expanded: they are only read
+    assert torch.equal(op.run(q[:1].expand(2, -1, -1, -1), ptab, 40), op.run(q[:1].repeat(2, 1, 1, 1), ptab, 40))
+    c.status()
