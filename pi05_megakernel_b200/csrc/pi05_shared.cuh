@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   __shared__ float2 s_ml[2][2][ROWS];       // at its end: the groups' references and sums
   __shared__ Segment s_seg[threads(FORMAT) / 32], s_ahead[8];      // a warp's segment; a softmax warp's next one
   __shared__ Walk s_walk;
-  __shared__ uint32_t s_lost[2][2][2];      // by group and turn: keys of a ragged tile whose values are not all numbers
+  __shared__ uint32_t s_lost[2][2][2];      // by group, and by turn of its ragged tiles: keys of one whose values are not all numbers
   __shared__ __align__(16) float s_ones[CODES ? TILE : 1];
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
     // ---- softmax: thread = query row, group = every second tile.  A wait that gave up lets the rest run through, with NaN as the result
     const int group = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t unit = 0, tile = 0, seg = 0;
+    uint32_t unit = 0, tile = 0, seg = 0, turn = 0;
     auto load_q = [&](const Segment& s, uint32_t seg) {
       load_queries<DIM>(p, s, row, lanes + TM_Q + seg % Q_BUFS * (DIM / 2));
       if (lane == 0) ptx::mbar_arrive(q_full + 8 * (seg % Q_BUFS));
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         // (`ragged`) the same for an infinity or a NaN among its values, and the rows that do see it get NaN
         const bool ragged = !CODES && own + i >= 0 && (own + i + 1) * TILE > all_see;
         if (!CODES && (ragged || (mask0 & mask1 & ~(bad0 | bad1)) != 0xffffffffu)) {
-          const uint32_t u = unit + v_unit(i, count), at = u % UNITS, turn = n >> 1 & 1;
+          const uint32_t u = unit + v_unit(i, count), at = u % UNITS;
           ok = ok && WAIT(kv_full + 8 * at, (u / UNITS) & 1, WAIT_KV_FULL);
           const uint32_t z0 = ~mask0 | bad0, z1 = ~mask1 | bad1, line = ring + at * UNIT;
           // a key's row by D / 8 lanes, sixteen keys a warp
@@ -814,7 +814,9 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             if (mine_clear >> c & 1)
               ptx::st_shared_v4(line + (lane % (DIM / 8) >> 3) * (TILE * 128) + (16 * quad + c) * 128 + (lane & 7) * 16, 0u, 0u, 0u, 0u);
           if (ragged) {
-            if (row < 2) s_lost[group][turn ^ 1][row] = 0u;                // (the group's last tile but one: everybody is through with it)
+            // The next ragged tile's, whatever tiles and items lie between: the last one that used it is an earlier tile of the group, whose product
+            // needed all four warps to be through with it and has been waited for above
+            if (row < 2) s_lost[group][turn ^ 1][row] = 0u;
 #pragma unroll 1
             for (int c = row; c < TILE * DIM / 8; c += 128) {
               const int key = c & 63, chunk = c >> 6;
@@ -836,6 +838,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           if (ragged) {
             ptx::named_bar_sync(LOST + group, 128);
             if ((k0 & s_lost[group][turn][0]) | (k1 & s_lost[group][turn][1])) l = __uint_as_float(0x7fffffffu);
+            turn ^= 1;
           }
         }
         __syncwarp();
