@@ -607,6 +607,8 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             const unsigned n0 = __ballot_sync(0xffffffffu, !f0), n1 = __ballot_sync(0xffffffffu, !f1);
             float top = fmaxf(f0 ? v0 : 0.f, f1 ? v1 : 0.f);
             for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            ptx::fence_proxy_async_shared();  // a later copy writes where these zeros went
+            __syncwarp();                     // (and lane 0 reports for all)
             if (lane == 0) {
               s_vlog[slot] = fmaxf(__log2f(top), -92.f) - 7.f;       // (of zeros: sums up to 2^99 a key have room in FP32)  7: see the softmax
               s_bad[slot][0] = info.bad[0] | n0;

@@ -67,3 +67,23 @@ def test_sequences_of_many_lengths(dim, q_heads, heads):
         sees[seq, tokens - 1, group * head:group * (head + 1)] = True
         assert bool(torch.isnan(got[sees]).all()) and torch.equal(got[~sees], clean[~sees]), seq
     op.status()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_cleared_scales_do_not_meet_later_copies(fmt, dim):
+    """Runs of many more tiles than there are buffers for scales, every third tile with scales that do not count (NaN in memory) and are cleared in place: the
+    same outputs whatever memory holds there, time after time."""
+    from pi05_megakernel_b200.shared import SharedPrefixAttention
+    batch, heads, own = 96, 8, 130
+    c, ptab, tab, lengths, rnd = filled(fmt, batch, 1, heads, dim, 640, own, seed=3)
+    q = rnd(batch, 1, 16, dim)
+    op = SharedPrefixAttention(c, 16, batch)
+    want, want_lse = op.run(q, ptab, 640, tab, lengths, with_lse=True)
+    assert bool(torch.isfinite(want).all())
+    for n in ("k", "v"):
+        getattr(c, n + "_scale")[tab[:, 2].long(), :, :, own - 128:] = float("nan")
+    for _ in range(40):
+        got, lse = op.run(q, ptab, 640, tab, lengths, with_lse=True)
+        assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    op.status()
