@@ -368,8 +368,9 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
  * over at most 2^30 tokens.
  * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8; query head h uses KV head
  * h / (q_heads / kv_heads).  lse (NULL: not wanted): [batch][tokens][q_heads] FP32, the logarithm of the sum of exp(scale q . k_j).
- * table = NULL: no own tokens.  Scores, softmax and sums are FP32; probabilities are rounded to BF16 (times the value's scale, 8 bits)
- * before the product with the values.  A bad page makes the queries that see it NaN; lengths[b] out of range is cut to the nearest
+ * table = NULL: no own tokens.  Scores, softmax and sums are FP32.  Before the product with the values a probability is rounded to BF16 (2^-8 of it); of an
+ * 8-bit cache its product with the value's scale to FP16: 2^-11 of it, or 2^-32 of the largest such product among the keys that the query sees where that is
+ * more (so for scales of values from 2^-80 to 2^90, those that are 0 aside).  A bad page makes the queries that see it NaN; lengths[b] out of range is cut to the nearest
  * that is in it; both are reported in the status words of the cache. */
 typedef struct pi05_shared_call {
   const void* q;

@@ -14,12 +14,13 @@
 //   * Warp 0 copies (TMA), warp 1 issues the MMAs, warp 2 looks pages and masks up ahead of both.  Two groups of four warps are the softmax, a
 //     thread per query row, and take the tiles in turn: what a tile costs a group is mostly latency (tensor memory, barriers, the special
 //     functions of one warp per scheduler), which the other group's tile hides.  They share the reference m of a row, which goes from tile to
-//     tile in order; it only moves when a score is more than 2^RESCALE above it, and then the row's sums in tensor memory are rescaled.
+//     tile in order; it only moves when an exponent to the base 2 is more than RESCALE above it, and then the row's sums in tensor memory are rescaled.
 //   * Of an 8-bit cache two more groups turn codes into 16 bits, exactly: keys into BF16, as the queries are, values into FP16.  A key's scale
-//     multiplies its score and a value's scale its probability, both in FP32.  The product, rounded to FP16, keeps four bits more than
-//     BF16 would; so that it stays in FP16's range whatever the scales are, the reference of a row takes in the largest scale of
-//     the tile (warp 3 finds it): a shift that the division by the row's sum takes out again.  (In BF16 the outputs were 0.0025 off the definition, relative to
-//     0.0017 of their own rounding; now 0.0017.)
+//     multiplies its score and a value's scale its probability, both in FP32.  The product, rounded to FP16, keeps three bits more than
+//     BF16 would; so that it stays in FP16's range whatever the scales are, the reference of a row is the largest exponent of such a product, of a key that
+//     the row sees: max_j (y_j + log2 s_j), with the logarithms of the values' scales by warp 3, once a tile.  A shift that the division by the row's sum
+//     takes out again.  What is below 2^-21 of the row's largest product loses bits to FP16's subnormals.  (In BF16 the outputs were 0.0025 off the definition,
+//     relative to 0.0017 of their own rounding; now 0.0017.)
 //
 // What bounds it (one B200, both kernels): 64 sequences over 16384 tokens in BF16 78 us beside 31 of HBM, 224 MB read at 2.9 TB/s, tensor pipe 24%: the chain of a tile
 // through one group (2800 cycles for 64 keys) and the latency of 512 short items; drafts in e4m3 121 us beside 21 of tensor pipe: instructions of softmax and
@@ -44,12 +45,16 @@ constexpr int BATCH = 8;                    // rounds of
 __host__ __device__ constexpr int overhead(int format) { return format == PI05_CACHE_BF16 ? 3 : 5; }
 constexpr int MAX_BATCH = 1024;
 constexpr float RESCALE = 8.0f;             // of exponents to the base 2: probabilities up to 256, their sums far from the ends of FP32
+// Of 8 bits: what is added to the logarithm of a value's scale, so that its products with probabilities are up to 2^7, 2^15 before the reference moves; and
+// the smallest such logarithm, which keeps 2^30 probabilities of up to 2^(80 + 7 + 8) in FP32 (of values below 1e-22 bits are lost instead).
+constexpr float LOG_SHIFT = -7.0f, LOG_LEAST = -80.0f;
 
 __host__ __device__ constexpr int unit_bytes(int dim) { return TILE * dim * 2; }
 // Units (64 keys or values) of the BF16 ring and of the ring of codes in front of it.
 __host__ __device__ constexpr int units(int format, int dim) { return format == PI05_CACHE_BF16 ? (dim == 256 ? 6 : 12) : dim == 256 ? 4 : 8; }
 __host__ __device__ constexpr int raw_units(int format, int dim) { return format == PI05_CACHE_BF16 ? 0 : dim == 256 ? 4 : 8; }
-__host__ __device__ constexpr int scale_bytes(int format) { return format == PI05_CACHE_BF16 ? 0 : INFO * 2 * TILE * 4; }
+// Of a tile: its keys' scales, its values', and the logarithms of the latter.
+__host__ __device__ constexpr int scale_bytes(int format) { return format == PI05_CACHE_BF16 ? 0 : INFO * 3 * TILE * 4; }
 __host__ __device__ constexpr int smem_bytes(int format, int dim) {
   return units(format, dim) * unit_bytes(dim) + raw_units(format, dim) * TILE * dim + scale_bytes(format) + (2 * MAX_BATCH + 1) * 4 + 1024;
 }
@@ -306,7 +311,6 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[4 * INFO + 2 * UNITS + 2 * RAW + Q_BUFS + 2 * S_BUFS + 5];
   __shared__ Info s_info[INFO];
-  __shared__ float s_vlog[INFO];            // log2 of the largest scale of a tile's values
   __shared__ uint32_t s_bad[INFO][2];       // Info::bad and the keys whose value's scale is not a number
   __shared__ float s_ref[2][ROWS];          // the rows' references, by segment
   __shared__ float2 s_ml[2][2][ROWS];       // at its end: the groups' references and sums
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
               if constexpr (CODES) {
                 ptx::tma_load_4d(dst + j * p.piece * DIM, map, full, 0, in, h, page);
                 if (!is_v) {
-                  const uint32_t to = scales + (slot * 2 * TILE + j * p.piece) * 4;
+                  const uint32_t to = scales + (slot * 3 * TILE + j * p.piece) * 4;
                   bulk_load(to, p.c.k_scale + info.scale[j], p.piece * 4, scale_full + 8 * slot);
                   bulk_load(to + TILE * 4, p.c.v_scale + info.scale[j], p.piece * 4, scale_full + 8 * slot);
                 }
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           p.parts[item] = part;
         }
       }
-      // ---- the largest scale of a tile's values that count
+      // ---- a tile's scales: of the keys times the softmax's constant, of the values at places that count, and the logarithms of those
       if constexpr (CODES) {
         uint32_t tile = 0;
         while (ok && NEXT) {
@@ -596,23 +600,26 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             ok = WAIT(info_full + 8 * slot, (n / INFO) & 1, WAIT_INFO);
             if (ok) ok = WAIT(scale_full + 8 * slot, (n / INFO) & 1, WAIT_SCALES);
             if (!ok) break;
-            float* vs = const_cast<float*>(s_scales) + (slot * 2 + 1) * TILE;
+            float* ks = const_cast<float*>(s_scales) + slot * 3 * TILE;
             const Info& info = s_info[slot];
-            const bool c0 = (info.mask[0] & ~info.bad[0]) >> lane & 1, c1 = (info.mask[1] & ~info.bad[1]) >> lane & 1;
-            const float v0 = c0 ? vs[lane] : 0.f, v1 = c1 ? vs[lane + 32] : 0.f;
-            // a scale that does not count is whatever memory holds, and 0 x NaN is NaN: zero in its place, also where it counts and is not a number
-            const bool f0 = fabsf(v0) < INFINITY, f1 = fabsf(v1) < INFINITY;
-            if (!c0 || !f0) vs[lane] = 0.f;
-            if (!c1 || !f1) vs[lane + 32] = 0.f;
-            const unsigned n0 = __ballot_sync(0xffffffffu, !f0), n1 = __ballot_sync(0xffffffffu, !f1);
-            float top = fmaxf(f0 ? v0 : 0.f, f1 ? v1 : 0.f);
-            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            unsigned none[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float *k = ks + 32 * half + lane, *v = k + TILE;
+              const bool counts = (info.mask[half] & ~info.bad[half]) >> lane & 1;
+              const float s = counts ? *v : 0.f;
+              // a scale that does not count is whatever memory holds, and 0 x NaN is NaN: zero in its place, also where it counts and is not a number
+              const bool finite = fabsf(s) < INFINITY;
+              none[half] = __ballot_sync(0xffffffffu, !finite);
+              if (!counts || !finite) *v = 0.f;
+              *k *= p.c_log2;               // (a score then is an exponent to the base 2 by one product)
+              v[TILE] = fmaxf(__log2f(finite ? fabsf(s) : 0.f), LOG_LEAST) + LOG_SHIFT;
+            }
             ptx::fence_proxy_async_shared();  // a later copy writes where these zeros went
             __syncwarp();                     // (and lane 0 reports for all)
             if (lane == 0) {
-              s_vlog[slot] = fmaxf(__log2f(top), -92.f) - 7.f;       // (of zeros: sums up to 2^99 a key have room in FP32)  7: see the softmax
-              s_bad[slot][0] = info.bad[0] | n0;
-              s_bad[slot][1] = info.bad[1] | n1;
+              s_bad[slot][0] = info.bad[0] | none[0];
+              s_bad[slot][1] = info.bad[1] | none[1];
               ptx::mbar_arrive(vlog_full + 8 * slot);
               ptx::mbar_arrive(info_empty + 8 * slot);
             }
@@ -680,7 +687,9 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         const bool special = __any_sync(0xffffffffu, (k0 & k1) != 0xffffffffu);
         ok = ok && WAIT(s_full + 8 * sbuf, (n / S_BUFS) & 1, WAIT_S);
         ptx::tc_fence_after();
-        const float4* ks = reinterpret_cast<const float4*>(s_scales + slot * 2 * TILE);
+        const float4* ks = reinterpret_cast<const float4*>(s_scales + slot * 3 * TILE);
+        // Of 8 bits: what turns a score into an exponent, the first time and, where keys that do not count are marked, the second
+        const float4* scale = special ? reinterpret_cast<const float4*>(s_ones) : ks;
         const uint32_t s_at = lanes + TM_S + sbuf * TILE, p_at = lanes + TM_P + buf * P_STEP;
         // A tile is read twice, CHUNK scores at a time: for the row's maximum, then for the probabilities.  (What the warps of a CTA execute per tile has to fit the
         // instruction cache.  With all 64 scores in registers 26% of the fetches missed it and drafts, 32 x 8 over 8192 in e4m3, took 245 us; read
@@ -696,20 +705,29 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           for (int h = 0; h < TILE; h += CHUNK) {
             float x[CHUNK];
             load_chunk(s_at + h, x);
-            if (CODES) {
+            if (special) {                  // keys that do not count: -infinity, there (of 8 bits exponents) for the second time too
+              if (CODES) {
 #pragma unroll
-              for (int j = 0; j < CHUNK; j += 4) {
-                const float4 f = ks[(h + j) / 4];
-                const float2 y = mul2(make_float2(x[j], x[j + 1]), make_float2(f.x, f.y)), z = mul2(make_float2(x[j + 2], x[j + 3]), make_float2(f.z, f.w));
-                x[j] = y.x; x[j + 1] = y.y; x[j + 2] = z.x; x[j + 3] = z.y;
+                for (int j = 0; j < CHUNK; j += 4) {
+                  const float4 f = ks[(h + j) / 4];
+                  const float2 y = mul2(make_float2(x[j], x[j + 1]), make_float2(f.x, f.y)), z = mul2(make_float2(x[j + 2], x[j + 3]), make_float2(f.z, f.w));
+                  x[j] = y.x; x[j + 1] = y.y; x[j + 2] = z.x; x[j + 3] = z.y;
+                }
               }
-            }
-            if (special) {                  // keys that do not count: -infinity, there (scaled) for the second time too
               const uint32_t k = (h < 32 ? k0 : k1) >> (h & 31);
 #pragma unroll
               for (int j = 0; j < CHUNK; ++j) x[j] = k >> j & 1 ? x[j] : -INFINITY;
 #pragma unroll
               for (int j = 0; j < CHUNK; j += 8) ptx::tmem_st_32x8(s_at + h + j, reinterpret_cast<uint32_t(&)[8]>(x[j]));
+            }
+            if (CODES) {                    // exponents of the products of probability and value's scale
+#pragma unroll
+              for (int j = 0; j < CHUNK; j += 4) {
+                const float4 f = scale[(h + j) / 4], v = ks[(2 * TILE + h + j) / 4];
+                const float2 y = ptx::fma2(make_float2(x[j], x[j + 1]), make_float2(f.x, f.y), make_float2(v.x, v.y)),
+                             z = ptx::fma2(make_float2(x[j + 2], x[j + 3]), make_float2(f.z, f.w), make_float2(v.z, v.w));
+                x[j] = y.x; x[j + 1] = y.y; x[j + 2] = z.x; x[j + 3] = z.y;
+              }
             }
             float a = high, b = -INFINITY;
 #pragma unroll
@@ -720,8 +738,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
             high = fmaxf(a, b);
           }
           if (special) ptx::tmem_wait_st();
-          high *= p.c_log2;
-          if (CODES) high += s_vlog[slot];  // largest exponent of a probability times its value's scale, or a little more; 7 less: products up to 2^15 at 2^RESCALE
+          if (!CODES) high *= p.c_log2;
           bool write = true;
           if (i == 0) {
             m = high;
@@ -764,7 +781,6 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
           const float ref = m == -INFINITY ? 0.f : m;
           const float2 c2 = make_float2(p.c_log2, p.c_log2), r2 = make_float2(-ref, -ref);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          const float4* scale = special ? reinterpret_cast<const float4*>(s_ones) : ks;
 #pragma unroll 1
           for (int h = 0; h < TILE; h += CHUNK) {
             float x[CHUNK];
@@ -773,13 +789,13 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
 #pragma unroll
             for (int j = 0; j < CHUNK; j += 4) {
               float2 e = make_float2(x[j], x[j + 1]), f = make_float2(x[j + 2], x[j + 3]);
+              float2 ce = c2, cf = c2;
               if (CODES) {
                 const float4 s = scale[(h + j) / 4];
-                e = mul2(e, make_float2(s.x, s.y));
-                f = mul2(f, make_float2(s.z, s.w));
+                ce = make_float2(s.x, s.y); cf = make_float2(s.z, s.w);
               }
-              e = ptx::fma2(e, c2, r2);
-              f = ptx::fma2(f, c2, r2);
+              e = ptx::fma2(e, ce, r2);
+              f = ptx::fma2(f, cf, r2);
               e.x = ptx::ex2_approx(e.x); e.y = ptx::ex2_approx(e.y); f.x = ptx::ex2_approx(f.x); f.y = ptx::ex2_approx(f.y);
               sum[0] = add2(sum[0], e);
               sum[1] = add2(sum[1], f);
