@@ -353,8 +353,13 @@ typedef struct pi05_cache_rows {
  * scale NaN and reads back as NaN.  Rows behind counts[b] stay as they are.  Two rows of one call for the same place of the cache: either, or their
  * codes and scales mixed. */
 int pi05_cache_write(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
-/* Rows out of their pages (k and v are written): code x scale in FP32, rounded to BF16.  Zeros behind counts[b]; NaN where a page or position is bad. */
+/* Rows out of their pages (k and v are written): code x scale in FP32, rounded to BF16.  Zeros behind counts[b]; NaN where a page or position is bad.
+ * No two rows that are written may meet (pi05_rows_meet), k's and v's neither: PI05_ERR_ARGUMENT. */
 int pi05_cache_read(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream);
+/* On the host: whether rows of `width` elements of two tensors meet, one at i . stride_a (i[k] < size_a[k], k < dims <= 4), the other at distance + j . stride_b,
+ * all in elements; size_b = NULL: whether two different rows of the first tensor do.  Returns 0: none do, 1: some do (or strides so tangled that it cannot
+ * be told in 10000 steps). */
+int pi05_rows_meet(int dims, const long long* size_a, const long long* stride_a, const long long* size_b, const long long* stride_b, long long distance, int width);
 /* Waits for `stream`, reads and clears the status words: PI05_ERR_PAGE_TABLE with code = PI05_CACHE_BAD_* and where = the
  * sequence, PI05_ERR_DEVICE_TIMEOUT with code = the kind of wait and where = block << 16 (the call's outputs are NaN then), or PI05_OK. */
 int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* code, int* where);
@@ -366,7 +371,8 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
  * are not finite (all of its outputs are NaN where other queries of the sequence do not see it).  A query without any key gets zeros and lse -infinity.
  * At most 1024 sequences and 2^27 query rows (batch x tokens x q_heads) a call.  A prefix, and a row of the table, reaches
  * over at most 2^30 tokens.
- * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8; query head h uses KV head
+ * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8, no row of out on another one or on one of q
+ * (pi05_rows_meet: PI05_ERR_ARGUMENT); query head h uses KV head
  * h / (q_heads / kv_heads).  lse (NULL: not wanted): [batch][tokens][q_heads] FP32, the logarithm of the sum of exp(scale q . k_j).
  * table = NULL: no own tokens.  Scores, softmax and sums are FP32.  Before the product with the values a probability is rounded to BF16 (2^-8 of it); of an
  * 8-bit cache its product with the value's scale to FP16: 2^-11 of it, or 2^-32 of the largest such product among the keys that the query sees where that is

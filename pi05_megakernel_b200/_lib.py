@@ -133,6 +133,8 @@ SIGNATURES = {
     "pi05_prefill_destroy": (_c.c_int, [_c.c_void_p]),
     "pi05_cache_write": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.c_void_p]),
     "pi05_cache_read": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.c_void_p]),
+    "pi05_rows_meet": (_c.c_int, [_c.c_int, _c.POINTER(_c.c_longlong), _c.POINTER(_c.c_longlong), _c.POINTER(_c.c_longlong), _c.POINTER(_c.c_longlong),
+                                  _c.c_longlong, _c.c_int]),
     "pi05_cache_status": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
     "pi05_shared_workspace": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
     "pi05_shared_attention": (_c.c_int, [_c.c_int, _c.POINTER(Cache), _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),

@@ -55,6 +55,18 @@ def strides(t: torch.Tensor) -> list[int]:
     return [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
 
 
+def meet(lib, a: torch.Tensor, b: torch.Tensor | None = None) -> bool:
+    """Whether two rows (along the last dimension) of a tensor lie on one another, or one of ``a`` and one of ``b``."""
+    numbers = lambda v: (ctypes.c_longlong * len(v))(*v)
+    other = (None, None, 0) if b is None else (numbers(b.shape[:-1]), numbers(strides(b)), (b.data_ptr() - a.data_ptr()) // a.element_size())
+    return bool(lib.pi05_rows_meet(a.dim() - 1, numbers(a.shape[:-1]), numbers(strides(a)), *other, a.shape[-1]))
+
+
+def span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) if t.numel() else 0
+
+
 class KvCache:
     """``pages`` pages of ``page_tokens`` tokens (a multiple of 16) for ``layers`` layers and ``kv_heads`` heads of ``head_dim`` (64, 128 or 256)
     elements; ``format`` is ``"bf16"``, ``"int8"`` or ``"e4m3"``.
@@ -142,6 +154,17 @@ class KvCache:
             raise ValueError("k and v must share their strides (multiples of 8 elements, the last dimension contiguous) and be 16-byte aligned")
         return ROWS.pack(kp, vp, *fit[:4], table.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), *fit[4:])
 
+    def _apart(self, k, v) -> None:
+        """Refuses outputs that several blocks would write at once."""
+        key = ("out", k.shape, k.stride())
+        reach = self.fits.get(key)
+        if reach is None:
+            if meet(self.lib, k):
+                raise ValueError("the rows of out must lie in different places")
+            reach = self.fits[key] = span(k)
+        if abs(k.data_ptr() - v.data_ptr()) < reach and meet(self.lib, k, v):
+            raise ValueError("the rows of out must lie in different places")
+
     def write(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, starts: torch.Tensor | None = None,
               counts: torch.Tensor | None = None, layer: int = 0) -> None:
         """Rows into their pages, asynchronous on the current stream.  ``k``, ``v`` BF16 ``[batch, layers, tokens, kv_heads, head_dim]`` of any
@@ -155,17 +178,20 @@ class KvCache:
     def read(self, table: torch.Tensor, tokens: int, starts: torch.Tensor | None = None, counts: torch.Tensor | None = None, layer: int = 0,
              layers: int | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows out of their pages, asynchronous on the current stream: BF16 keys and values ``[batch, layers, tokens, kv_heads, head_dim]`` of
-        layers ``layer`` .. (all that there are), zeros behind ``counts[b]``; the rest as in ``write``."""
+        layers ``layer`` .. (all that there are), zeros behind ``counts[b]``; the rest as in ``write``.  The rows of ``out`` lie in different places, those of
+        keys and of values too."""
         if layers is None:
             layers = self.layers - layer
-        if out is None:
+        given = out is not None
+        if not given:
             shape = (table.shape[0], layers, tokens, self.kv_heads, self.head_dim)
             out = (self.fresh(shape, torch.bfloat16), self.fresh(shape, torch.bfloat16))
         elif out[0].shape[1:3] != (layers, tokens):
             raise ValueError("out does not have the layers and tokens that are read")
-        elif any(s == 0 and n > 1 for n, s in zip(out[0].shape, out[0].stride())):
-            raise ValueError("the rows of out must lie in different places")
-        rc = self.call_read(self.index, self.ref, self._rows(*out, table, starts, counts, layer), raw_stream(self.index))
+        rows = self._rows(*out, table, starts, counts, layer)
+        if given:
+            self._apart(*out)
+        rc = self.call_read(self.index, self.ref, rows, raw_stream(self.index))
         if rc:
             _lib.check(self.lib, None, rc)
         return out

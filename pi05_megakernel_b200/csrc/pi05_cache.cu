@@ -206,7 +206,7 @@ struct DeviceGuard {
   ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
 };
 
-int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c, const pi05_cache_rows* r, void* stream) {
+int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c, const pi05_cache_rows* r, void* stream, bool out) {
   if (device < 0 || !cache::well_formed(c) || !r) return PI05_ERR_ARGUMENT;
   if (r->batch < 0 || r->tokens < 0 || r->layers < 0 || r->layer < 0 || r->layer > c->layers - r->layers || r->table_pages < 0 || r->table_stride < 0)
     return PI05_ERR_ARGUMENT;
@@ -216,6 +216,12 @@ int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c,
   if ((((uintptr_t)r->k | (uintptr_t)r->v) & 15) || ((r->batch_stride | r->layer_stride | r->token_stride | r->head_stride) & 7) ||
       (((uintptr_t)r->table | (uintptr_t)r->starts | (uintptr_t)r->counts) & 3))
     return PI05_ERR_ARGUMENT;
+  if (out) {                                                       // rows on one another would be written by several blocks at once
+    const long long size[4] = {r->batch, r->layers, r->tokens, c->kv_heads}, stride[4] = {r->batch_stride, r->layer_stride, r->token_stride, r->head_stride};
+    const long long apart = (long long)((intptr_t)r->v - (intptr_t)r->k) / 2;
+    if (cache::rows_meet(4, size, stride, nullptr, nullptr, 0, c->head_dim) || cache::rows_meet(4, size, stride, size, stride, apart, c->head_dim))
+      return PI05_ERR_ARGUMENT;
+  }
   DeviceGuard guard(device);
   if (!guard.ok) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }
   const int per = BLOCK / (c->head_dim / 16);
@@ -231,12 +237,18 @@ int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c,
 
 extern "C" {
 
+int pi05_rows_meet(int dims, const long long* size_a, const long long* stride_a, const long long* size_b, const long long* stride_b, long long distance,
+                   int width) {
+  if (dims < 0 || dims > 4 || width < 1 || !size_a || !stride_a || (size_b && !stride_b)) return 1;
+  return cache::rows_meet(dims, size_a, stride_a, size_b, stride_b, distance, width) ? 1 : 0;
+}
+
 int pi05_cache_write(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream) {
-  return move_rows(kWrite, device, cache, rows, stream);
+  return move_rows(kWrite, device, cache, rows, stream, false);
 }
 
 int pi05_cache_read(int device, const pi05_cache* cache, const pi05_cache_rows* rows, void* stream) {
-  return move_rows(kRead, device, cache, rows, stream);
+  return move_rows(kRead, device, cache, rows, stream, true);
 }
 
 int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* code, int* where) {

@@ -66,6 +66,57 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Host: whether rows of `width` elements meet, one at i . stride_a (i_k < size_a[k]) and the other at distance + j . stride_b; with size_b = NULL
+// two different rows of the first tensor.  A row's place is a sum of terms stride x index, so this asks for indexes that bring such a sum into (-width, width):
+// largest stride first, of whose indexes only those are tried that the smaller strides can still make up for, one to three where strides are nested.
+struct MeetTerm { long long stride, lo, hi; };
+inline bool meet_search(const MeetTerm* t, int terms, __int128 at, long long width, bool other, bool moved, int* budget) {
+  if (--*budget < 0) return true;                                  // cannot be told: as if they met
+  if (terms == 0) return at < width && at > -(__int128)width && (other || moved);
+  __int128 lo = 0, hi = 0;                                         // what the smaller strides reach
+  for (int i = 1; i < terms; ++i) { lo += (__int128)t[i].stride * t[i].lo; hi += (__int128)t[i].stride * t[i].hi; }
+  auto down = [&](__int128 v) { return v >= 0 ? v / t->stride : -((-v + t->stride - 1) / t->stride); };
+  __int128 first = -down(width - 1 + at + hi), last = down(width - 1 - at - lo);
+  if (first < t->lo) first = t->lo;
+  if (last > t->hi) last = t->hi;
+  for (__int128 x = first; x <= last; ++x)
+    if (meet_search(t + 1, terms - 1, at + x * t->stride, width, other, moved || x != 0, budget)) return true;
+  return false;
+}
+inline bool rows_meet(int dims, const long long* size_a, const long long* stride_a, const long long* size_b, const long long* stride_b, long long distance,
+                      long long width) {
+  MeetTerm t[8];
+  int n = 0;
+  const bool other = size_b != nullptr;
+  for (int k = 0; k < dims; ++k)
+    if (size_a[k] <= 0 || (other && size_b[k] <= 0)) return false; // no rows
+  for (int side = 0; side < (other ? 2 : 1); ++side)
+    for (int k = 0; k < dims; ++k) {
+      const long long size = (side ? size_b : size_a)[k], stride = (side ? stride_b : stride_a)[k];
+      if (size == 1 || (stride == 0 && other)) continue;
+      if (stride == 0) return true;
+      const bool up = (side != 0) == (stride > 0);                 // (of the first tensor the index is subtracted)
+      MeetTerm term = {stride < 0 ? -stride : stride, other && up ? 0 : -(size - 1), other && !up ? 0 : size - 1};
+      int at = 0;
+      while (at < n && t[at].stride > term.stride) ++at;
+      if (at < n && t[at].stride == term.stride) {
+        if (!other) return true;
+        t[at].lo += term.lo; t[at].hi += term.hi;
+        continue;
+      }
+      for (int i = n++; i > at; --i) t[i] = t[i - 1];
+      t[at] = term;
+    }
+  if (!other) {                                                    // every stride behind all that the smaller ones reach: as tensors usually lie
+    __int128 extent = width;
+    int i = n;
+    while (i > 0 && t[i - 1].stride >= extent) { --i; extent += (__int128)t[i].stride * t[i].hi; }
+    if (i == 0) return false;
+  }
+  int budget = 10000;
+  return meet_search(t, n, distance, width, other, false, &budget);
+}
+
 // Host: whether a cache is one that the kernels can work on.
 inline bool well_formed(const pi05_cache* c) {
   if (!c || !c->k || !c->v || !c->status) return false;

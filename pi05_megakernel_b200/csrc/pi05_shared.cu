@@ -78,6 +78,12 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   if (s.batch > shared::MAX_BATCH || (long long)s.batch * s.tokens * s.q_heads > 1ll << 27) return PI05_ERR_UNSUPPORTED;
   // places of keys are counted in 32 bits, in whole tiles: far enough from their end that rounding up does not pass it
   if (s.prefix_tokens > 1 << 30 || (s.table && (long long)s.table_pages * c.page_tokens > 1ll << 30)) return PI05_ERR_UNSUPPORTED;
+  {                                             // outputs on one another, or over queries that another CTA has yet to read
+    const long long size[3] = {s.batch, s.tokens, s.q_heads}, os[3] = {s.out_batch_stride, s.out_token_stride, s.out_head_stride},
+                    qs[3] = {s.q_batch_stride, s.q_token_stride, s.q_head_stride};
+    const long long apart = (long long)((intptr_t)s.out - (intptr_t)s.q) / 2;
+    if (cache::rows_meet(3, size, os, nullptr, nullptr, 0, c.head_dim) || cache::rows_meet(3, size, qs, size, os, apart, c.head_dim)) return PI05_ERR_ARGUMENT;
+  }
   DeviceGuard guard(device);
   int sms = 0;
   if (!guard.ok || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return PI05_ERR_NO_DEVICE; }

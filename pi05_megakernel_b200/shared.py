@@ -14,7 +14,7 @@ import struct
 import torch
 
 from . import _lib
-from .cache import MAX_FITS, KvCache, check_table, describe, raw_stream, strides
+from .cache import MAX_FITS, KvCache, check_table, describe, meet, raw_stream, span, strides
 
 CALL = struct.Struct("@PPP6qPPPP8if4x")      # pi05_shared_call of the header
 
@@ -47,16 +47,21 @@ class SharedPrefixAttention:
         ``scale`` defaults to head_dim ** -0.5.  A query that sees no key gets zeros (log-sum-exp: -infinity)."""
         key = (q.shape, q.stride(), q.dtype, q.device, describe(out), describe(prefix_table), prefix_tokens, describe(table), describe(lengths),
                describe(valid), layer, causal, scale)
-        if out is None:
+        given = out is not None
+        if not given:
             out = self.fresh(q.shape, torch.bfloat16)
-        fit = self.fits.get(key)
-        if fit is None:
+        known = self.fits.get(key)
+        if known is None:
             if len(self.fits) >= MAX_FITS:
                 self.fits.clear()
-            fit = self.fits[key] = self._fit(q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale)
+            fit = self._fit(q, out, prefix_table, prefix_tokens, table, lengths, layer, valid, causal, scale)
+            known = self.fits[key] = (fit, span(q), span(out))
+        fit, q_span, out_span = known
         qp, op = q.data_ptr(), out.data_ptr()
         if (qp | op) & 15:
             raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
+        if given and qp < op + out_span and op < qp + q_span and meet(self.lib, q, out):
+            raise ValueError("the rows of out must not lie over those of q")
         lse = self.fresh(q.shape[:3], torch.float32) if with_lse else None
         call = CALL.pack(qp, op, lse.data_ptr() if with_lse else 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0,
                          valid.data_ptr() if prefix_tokens and valid is not None else 0, 0 if table is None else table.data_ptr(),
@@ -82,7 +87,7 @@ class SharedPrefixAttention:
         qs, os_ = strides(q), strides(out)
         if q.stride(3) != 1 or out.stride(3) != 1 or any(s % 8 for s in qs + os_):
             raise ValueError("q and out need strides of multiples of 8 elements, a contiguous last dimension and 16-byte alignment")
-        if any(s == 0 and n > 1 for n, s in zip(out.shape, os_)):
+        if meet(self.lib, out):
             raise ValueError("the rows of out must lie in different places")
         if prefix_tokens:
             if prefix_table is None:
