@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .cache import KvCache
+from .cache import KvCache, check_table
 from .fixture import PREFILL_WEIGHTS, PrefillGeometry, prefill_shapes
 from .shared import CALL, SharedPrefixAttention
 
@@ -63,10 +63,15 @@ class Pi05Prefill:
     def run(self, embeddings: torch.Tensor, valid: torch.Tensor, layers: int | None = None,
             out: tuple[torch.Tensor, torch.Tensor] | None = None, cache: KvCache | None = None,
             table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """Asynchronous on the current stream.  ``embeddings`` [tokens, 2048] BF16, ``valid`` [tokens] bool.  With ``cache`` the keys and values also go
-        into the pages that ``table`` int32 [pages] names (``KvCache.write``)."""
+        """Asynchronous on the current stream.  ``embeddings`` [tokens, 2048] BF16, ``valid`` [tokens] bool.  With ``cache`` the keys and values of the
+        layers that run also go into the pages that ``table`` int32 [pages] names (``KvCache.write``)."""
+        count = self.geo.layers if layers is None else layers
         if (cache is None) != (table is None):
             raise ValueError("a cache needs the page table of the prompt, and a table its cache")
+        if cache is not None:
+            if cache.kv_heads != self.geo.kv_heads or cache.head_dim != self.geo.head_dim or cache.layers < count or cache.device != self.device:
+                raise ValueError(f"the cache must hold {count} layers of one KV head of 256 on {self.device}")
+            check_table("table", table, self.device, 1)
         tokens = embeddings.shape[0]
         if tuple(embeddings.shape) != (tokens, self.geo.hidden) or embeddings.dtype != torch.bfloat16 or \
                 tuple(valid.shape) != (tokens,) or valid.dtype != torch.bool:
@@ -81,9 +86,9 @@ class Pi05Prefill:
                                             make(shape, dtype=torch.bfloat16, device=self.device))
         stream = torch.cuda.current_stream(self.device).cuda_stream
         self._check(self.lib.pi05_prefill_run(self.handle, embeddings.data_ptr(), valid.data_ptr(), tokens, k.data_ptr(),
-                                              v.data_ptr(), self.geo.layers if layers is None else layers, stream))
-        if cache is not None:
-            cache.write(k[None], v[None], table[None])
+                                              v.data_ptr(), count, stream))
+        if cache is not None:                     # (of the other layers nothing: they may be those of an earlier run)
+            cache.write(k[None, :count], v[None, :count], table[None])
         return k, v
 
     def step(self, embeddings: torch.Tensor, positions: torch.Tensor, attention: SharedPrefixAttention, prefix_table: torch.Tensor | None,
