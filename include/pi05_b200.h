@@ -322,7 +322,8 @@ int pi05_prefill_destroy(pi05_prefill_t h);
  *
  * A cache is two pools, keys and values, [pages][layers][page_tokens][kv_heads][head_dim]; head_dim 64, 128 or 256, page_tokens a multiple
  * of 16, pools and scales 16-byte aligned.  Formats: BF16; int8 and e4m3 with one FP32 scale per (token, head), [pages][layers][kv_heads]
- * [page_tokens]: the value of an element is code x scale.  A sequence is a row of an int32 page table in device memory: its token t lies in page
+ * [page_tokens]: the value of an element is code x scale.  A row that is not a number has a NaN as its scale; e4m3's two NaN codes are none of the format's (the
+ * library never writes them; they would count as +-480).  A sequence is a row of an int32 page table in device memory: its token t lies in page
  * table[t / page_tokens] at t % page_tokens.  Tables, starts, counts and lengths are read by the kernels when they run, so they may change
  * between launches and replays.  What they hold is checked there: the access is left out, and the status words of the cache (16 bytes of
  * device memory, zero before the first call) keep the first such code and the sequence it came from (-1: the shared prefix).  Several calls on one cache may run at once where

@@ -9,6 +9,7 @@ current stream; the work is done by ``libpi05_b200.so``.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 
 import torch
@@ -91,9 +92,17 @@ class KvCache:
 
     @classmethod
     def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> "KvCache":
-        """A cache over pools that exist already (the shapes above, contiguous)."""
+        """A cache over pools that exist already (the shapes above, contiguous).  The format has no e4m3 NaNs: a row that is not a number has a NaN as its
+        scale, which is what ``write`` gives it, and rows that hold such codes (0x7f, 0xff) now get one here.  Pools that something else writes later have to be
+        wrapped again."""
         self = cls.__new__(cls)
         self._set(k, v, k_scale, v_scale)
+        if self.format == "e4m3":
+            with torch.no_grad():
+                for codes, scale in ((k, k_scale), (v, v_scale)):
+                    step = max(1, (1 << 26) // max(1, codes[0].numel()))
+                    for c, s in zip(codes.view(torch.uint8).split(step), scale.split(step)):
+                        s.masked_fill_(c.bitwise_and(127).amax(-1).eq(127).transpose(2, 3), math.nan)
         return self
 
     def _set(self, k, v, k_scale, v_scale) -> None:
