@@ -161,7 +161,8 @@ class KvCache:
         kp, vp = k.data_ptr(), v.data_ptr()
         if (kp | vp) & 15:
             raise ValueError("k and v must share their strides (multiples of 8 elements, the last dimension contiguous) and be 16-byte aligned")
-        return ROWS.pack(kp, vp, *fit[:4], table.data_ptr(), 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), *fit[4:])
+        # (a table without pages: a place that is never read, so that what its rows ask for is reported like any other)
+        return ROWS.pack(kp, vp, *fit[:4], table.data_ptr() or kp, 0 if starts is None else starts.data_ptr(), 0 if counts is None else counts.data_ptr(), *fit[4:])
 
     def _apart(self, k, v) -> None:
         """Refuses outputs that several blocks would write at once."""

@@ -119,7 +119,7 @@ class Pi05Prefill:
         hidden = torch.empty_like(embeddings)
         starts = lengths - tokens
         call = CALL.pack(0, 0, 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0, valid.data_ptr() if prefix_tokens and valid is not None else 0,
-                         table.data_ptr(), lengths.data_ptr(), *fit[6:])
+                         table.data_ptr() or lengths.data_ptr(), lengths.data_ptr(), *fit[6:])
         stream = torch.cuda.current_stream(self.device).cuda_stream
         self._check(self.lib.pi05_prefill_step(self.handle, c.ref, call, embeddings.data_ptr(), positions.data_ptr(), starts.data_ptr(), hidden.data_ptr(),
                                                self.geo.layers if layers is None else layers, attention.workspace, attention.nbytes, stream))

@@ -64,7 +64,8 @@ class SharedPrefixAttention:
             raise ValueError("the rows of out must not lie over those of q")
         lse = self.fresh(q.shape[:3], torch.float32) if with_lse else None
         call = CALL.pack(qp, op, lse.data_ptr() if with_lse else 0, *fit[:6], prefix_table.data_ptr() if prefix_tokens else 0,
-                         valid.data_ptr() if prefix_tokens and valid is not None else 0, 0 if table is None else table.data_ptr(),
+                         valid.data_ptr() if prefix_tokens and valid is not None else 0,
+                         0 if table is None else table.data_ptr() or lengths.data_ptr(),          # (a table without pages: its lengths are checked all the same)
                          0 if lengths is None else lengths.data_ptr(), *fit[6:])
         rc = self.call(self.index, self.cache.ref, call, self.workspace, self.nbytes, raw_stream(self.index))
         if rc:
