@@ -13,6 +13,7 @@
 
 namespace {
 
+using cache::DeviceGuard;
 using cache::hi16;
 using cache::lo16;
 using cache::pack2;
@@ -81,9 +82,10 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
 
 // Sixteen elements of a row as codes, and the row's scale.
 //   code = rn(x * peak / a) of the true quotient, a the row's largest magnitude.  With BF16 x and a the quotient is either in the middle of
-// two codes exactly (x = a / 2 is 63.5) or at least 2^-10 away from it, so it only has to be right to that, and exact in the middle: peak / a as
-// the sum of two FP32 numbers (the reciprocal, a step of Newton's and what that leaves), and x times it as one FMA on top of the small product, which
-// rounds once.
+// two codes exactly (x = a / 2 is 63.5) or at least 2^-16 of itself away from it (int8: mantissas 254 and 255 give 126.502; e4m3: 2^-12.9; over all pairs of
+// mantissas), so it only has to be right to that, and exact in the middle: peak / a as the sum of two FP32 numbers (its approximation by the reciprocal,
+// corrected once by its residual, as Markstein, IBM J. Res. Dev. 34, 1990, and what the residual of that leaves), and x times it as one FMA on top of the
+// small product, which rounds once.  The scale a / peak is corrected by its residual in the same way.
 template <int FORMAT, int LANES>
 __device__ __forceinline__ uint4 encode(const uint4 (&x)[2], float* scale) {
   constexpr float PEAK = FORMAT == PI05_CACHE_INT8 ? 127.0f : 448.0f, ONE_PEAKTH = 1.0f / PEAK;
@@ -198,13 +200,6 @@ typedef void (*RowKernel)(const RowArgs);
 const RowKernel kWrite[3][3] = {BY_DIM(write_kernel, PI05_CACHE_BF16), BY_DIM(write_kernel, PI05_CACHE_INT8), BY_DIM(write_kernel, PI05_CACHE_E4M3)};
 const RowKernel kRead[3][3] = {BY_DIM(read_kernel, PI05_CACHE_BF16), BY_DIM(read_kernel, PI05_CACHE_INT8), BY_DIM(read_kernel, PI05_CACHE_E4M3)};
 #undef BY_DIM
-
-struct DeviceGuard {
-  int prev = -1;
-  bool ok;
-  explicit DeviceGuard(int dev) { if (cudaGetDevice(&prev) != cudaSuccess) prev = -1; ok = prev == dev || cudaSetDevice(dev) == cudaSuccess; }
-  ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
-};
 
 int move_rows(const RowKernel (&kernels)[3][3], int device, const pi05_cache* c, const pi05_cache_rows* r, void* stream, bool out) {
   if (device < 0 || !cache::well_formed(c) || !r) return PI05_ERR_ARGUMENT;

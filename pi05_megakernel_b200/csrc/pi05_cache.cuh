@@ -4,6 +4,7 @@
 // keys of one head as one vector, and a page's codes stay a dense box for tiled copies.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "../../include/pi05_b200.h"
@@ -116,6 +117,14 @@ inline bool rows_meet(int dims, const long long* size_a, const long long* stride
   int budget = 10000;
   return meet_search(t, n, distance, width, other, false, &budget);
 }
+
+// Host: `dev` as the current device, for as long as this lives.
+struct DeviceGuard {
+  int prev = -1;
+  bool ok;
+  explicit DeviceGuard(int dev) { if (cudaGetDevice(&prev) != cudaSuccess) prev = -1; ok = prev == dev || cudaSetDevice(dev) == cudaSuccess; }
+  ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
+};
 
 // Host: whether a cache is one that the kernels can work on.
 inline bool well_formed(const pi05_cache* c) {

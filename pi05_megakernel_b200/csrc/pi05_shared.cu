@@ -13,6 +13,7 @@
 
 namespace {
 
+using cache::DeviceGuard;
 using shared::Args;
 
 typedef void (*AttentionKernel)(const Args);
@@ -21,13 +22,6 @@ typedef void (*CombineKernel)(const Args, int);
 const AttentionKernel kAttention[3][3] = {BY_DIM(PI05_CACHE_BF16), BY_DIM(PI05_CACHE_INT8), BY_DIM(PI05_CACHE_E4M3)};
 #undef BY_DIM
 const CombineKernel kCombine[3] = {shared::combine_kernel<64>, shared::combine_kernel<128>, shared::combine_kernel<256>};
-
-struct DeviceGuard {
-  int prev = -1;
-  bool ok;
-  explicit DeviceGuard(int dev) { if (cudaGetDevice(&prev) != cudaSuccess) prev = -1; ok = prev == dev || cudaSetDevice(dev) == cudaSuccess; }
-  ~DeviceGuard() { if (prev >= 0) cudaSetDevice(prev); }
-};
 
 int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : 2; }
 long long up256(long long v) { return (v + 255) / 256 * 256; }

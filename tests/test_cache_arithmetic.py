@@ -1,4 +1,4 @@
-"""Rows of outputs that lie on one another are found on the host: against all pairs of rows, and what the entry points refuse."""
+"""Host arithmetic of the cache: rows of outputs that lie on one another are found, against all pairs of rows, and refused; how far quotients are from the middles of codes."""
 import ctypes
 import itertools
 import random
@@ -86,3 +86,26 @@ def test_entry_points_refuse(lib):
         assert lib.pi05_cache_write(0, cache(), rows(v=0x60000, token_stride=0), None) in fine
         for change in (dict(), dict(out=0x60000 + 2 * 2048), dict(q_batch_stride=0), dict(q_head_stride=0)):
             assert lib.pi05_shared_attention(0, cache(), call(**change), 0x100000, 1 << 30, None) in fine
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_quotients_of_codes_are_middles_or_far_from_them(fmt):
+    """What the one FP32 quotient of a write rests on: x peak / max|x| of two BF16 numbers is a middle of two codes exactly or at least 2^-16 (int8) and 2^-12.9 (e4m3) of
+    itself away from it.  In whole numbers, over all pairs of mantissas and all exponents that codes reach."""
+    import numpy as np
+    a, x = (v.ravel().astype(np.int64) for v in np.meshgrid(np.arange(128, 256), np.arange(128, 256)))
+    if fmt == "int8":
+        peak, down, middles = 127, range(0, 10), np.arange(1, 256, 2, dtype=np.int64) << 9          # in units of 2^-10
+    else:
+        peak, down = 448, range(0, 20)
+        values = np.array([m * 2 if e == 0 else (8 + m) << e for e, m in (divmod(c, 8) for c in range(127))], dtype=np.int64)      # of 2^-10
+        middles = (values[:-1] + values[1:]) // 2
+    nearest = np.inf
+    for e in down:
+        for i in (0, -1):
+            top = peak * x << 10                                          # quotient = top / (a << e), in the middles' units
+            at = np.clip(np.searchsorted(middles, top // (a << e)) + i, 0, len(middles) - 1)
+            off = np.abs(top - middles[at] * (a << e))
+            far = (off > 0) & (x <= a << e)                               # (x is not larger than max|x|)
+            nearest = min(nearest, (off[far] / top[far]).min())
+    assert nearest >= 2.0 ** (-16 if fmt == "int8" else -12.9), np.log2(nearest)
