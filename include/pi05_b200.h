@@ -368,8 +368,9 @@ int pi05_cache_status(int device, const pi05_cache* cache, void* stream, int* co
 /* Attention of batch x tokens queries over one prefix that all sequences share and over each sequence's own tokens:
  *   out = sum_j p_j v_j,  p = softmax(scale q . k_j)  over the prefix tokens j < prefix_tokens with prefix_valid[j] != 0 (NULL: all) and the own
  * tokens j < lengths[b] of sequence b; causal: own tokens j <= lengths[b] - tokens + t for query t, so that the queries are the last tokens
- * of the sequence.  What places of the cache hold that a query does not see does not matter to it; one that sees an infinity or a NaN gets outputs that
- * are not finite (all of its outputs are NaN where other queries of the sequence do not see it).  A query without any key gets zeros and lse -infinity.
+ * of the sequence.  What places of the cache hold that a query does not see does not matter to it.  One that sees a NaN, or a value that is infinite, gets
+ * outputs that are not finite (all of its outputs are NaN where other queries of the sequence do not see it); a key with infinities counts by its score: NaN for
+ * +infinity, and for -infinity it does not count.  A query without any key that counts gets zeros and lse -infinity.
  * At most 1024 sequences and 2^27 query rows (batch x tokens x q_heads) a call.  A prefix, and a row of the table, reaches
  * over at most 2^30 tokens.
  * q and out are BF16 [batch][tokens][q_heads][head_dim] with strides in elements, multiples of 8, no row of out on another one or on one of q

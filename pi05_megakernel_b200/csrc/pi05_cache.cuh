@@ -114,6 +114,9 @@ inline bool rows_meet(int dims, const long long* size_a, const long long* stride
     while (i > 0 && t[i - 1].stride >= extent) { --i; extent += (__int128)t[i].stride * t[i].hi; }
     if (i == 0) return false;
   }
+  __int128 lo = distance, hi = distance;                           // far apart: as tensors of their own are
+  for (int i = 0; i < n; ++i) { lo += (__int128)t[i].stride * t[i].lo; hi += (__int128)t[i].stride * t[i].hi; }
+  if (lo >= width || hi <= -width) return false;
   int budget = 10000;
   return meet_search(t, n, distance, width, other, false, &budget);
 }

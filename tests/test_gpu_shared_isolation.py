@@ -87,3 +87,28 @@ def test_cleared_scales_do_not_meet_later_copies(fmt, dim):
         got, lse = op.run(q, ptab, 640, tab, lengths, with_lse=True)
         assert torch.equal(got, want) and torch.equal(lse, want_lse)
     op.status()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_with_infinities(dim):
+    """BF16: a key counts by its score.  -infinity: as if it were masked, bit for bit, and zeros where no other key is left; +infinity: NaN."""
+    from pi05_megakernel_b200.shared import SharedPrefixAttention
+    c, ptab, tab, lengths, rnd = filled("bf16", 2, 1, 2, dim, 150, 20, seed=4)
+    q = rnd(2, 1, 4, dim)
+    q[..., 3] = torch.tensor([-1.0, -2.0, 1.0, 0.5], device="cuda")      # heads 0 and 1 see -infinity, 2 and 3 +infinity
+    op = SharedPrefixAttention(c, 4, 2)
+    for token in (0, 64, 149):
+        page, at = int(ptab[token // 64]), token % 64
+        old = c.k[page, 0, at].clone()
+        valid = torch.ones(150, dtype=torch.bool, device="cuda")
+        valid[token] = False
+        want, want_lse = op.run(q, ptab, 150, tab, lengths, valid=valid, with_lse=True)
+        c.k[page, 0, at, :, 3] = float("inf")
+        got, lse = op.run(q, ptab, 150, tab, lengths, with_lse=True)
+        c.k[page, 0, at] = old
+        assert torch.equal(got[:, :, :2], want[:, :, :2]) and torch.equal(lse[:, :, :2], want_lse[:, :, :2])
+        assert bool(torch.isnan(got[:, :, 2:]).all())
+    c.k[int(ptab[0]), 0, 0, :, 3] = float("inf")
+    got, lse = op.run(q, ptab, 1, with_lse=True)
+    assert bool((got[:, :, :2] == 0).all()) and bool((lse[:, :, :2] == -float("inf")).all()) and bool(torch.isnan(got[:, :, 2:]).all())
+    op.status()
