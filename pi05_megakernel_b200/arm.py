@@ -74,7 +74,8 @@ class PagedPrefix:
 
 class CachedPrefix:
     """The prefix cache in the pages of a ``KvCache`` of 18 layers and one KV head of 256, of any format: every launch reads it back to BF16 first
-    (what the pages and the table hold then).  ``table`` is an int32 tensor ``[batch, pages]`` on the cache's device."""
+    (what the pages and the table hold then).  ``table`` is an int32 tensor ``[batch, pages]`` on the cache's device; a page in it that does not exist
+    makes its observation's chunk NaN and is reported by the cache's ``status``."""
 
     def __init__(self, cache: KvCache, table: torch.Tensor) -> None:
         if cache.kv_heads != 1 or cache.head_dim != 256:

@@ -92,8 +92,10 @@ int pi05_shared_attention(int device, const pi05_cache* cache, const pi05_shared
   a.a_tiles = (int)k.a_tiles; a.b_tiles = (int)k.b_tiles; a.b_rows = (int)k.b_rows; a.b_slot = (int)k.b_slot;
   a.overhead = shared::overhead(c.format);
   a.p_tiles = (s.prefix_tokens + shared::TILE - 1) / shared::TILE;
-  // Prefix and own tokens as one list of keys where packing the batch's rows would not save a quarter of the tiles: eight times 50 tokens of 8 heads (32
-  // tiles, or 25 packed) over 968 29.2 us, packed 30.3
+  // Prefix and own tokens as one list of keys where packing the batch's rows would not save a quarter of the tiles.  8 heads of 256, one list / packed, in us
+  // (BF16; int8): 16 x 50 over 200 31.8 / 37.5; 34.9 / 36.4, over 968 40.3 / 42.8; 45.2 / 47.9, over 4000 60.9 / 67.7; 77.1 / 73.2.  8 x 50 over 968 26.3 / 26.7;
+  // 31.0 / 31.5, over 4000 39.8 / 40.5; 47.2 / 45.3.  Where packing saves more it still is up to 17% slower for a few sequences (8 x 20 over 968 23.1 / 24.4;
+  // 26.2 / 27.7, 2 x 8 over 200 13.2 / 15.5; 15.2 / 17.6), but it is what makes the prefix one pass for many of a token each
   a.joined = a.p_tiles == 0 || 3ll * s.batch * k.b_tiles <= 4 * k.a_tiles;
   const long long own = s.table ? ((long long)s.table_pages * c.page_tokens + shared::TILE - 1) / shared::TILE : 0;
   const long long most = c.kv_heads * ((a.joined ? 0 : k.a_tiles * (a.overhead + a.p_tiles)) +

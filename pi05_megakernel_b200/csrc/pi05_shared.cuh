@@ -23,7 +23,7 @@
 //     relative to 0.0017 of their own rounding; now 0.0017.)
 //
 // What bounds it (one B200, both kernels): 64 sequences over 16384 tokens in BF16 78 us beside 31 of HBM, 224 MB read at 2.9 TB/s, tensor pipe 24%: the chain of a tile
-// through one group (2800 cycles for 64 keys) and the latency of 512 short items; drafts in e4m3 121 us beside 21 of tensor pipe: instructions of softmax and
+// through one group (2800 cycles for 64 keys) and the latency of 512 short items; drafts in e4m3 122 us beside 21 of tensor pipe: instructions of softmax and
 // converters; steps of a few sequences 12 to 18 us: launch, lengths, page lookup, first bytes, one tile, its parts and the second kernel, one after the other.
 #pragma once
 #include <cuda.h>
@@ -39,9 +39,15 @@ constexpr int TILE = 64;                    // keys of a tile
 constexpr int ROWS = 128;                   // query rows of a tile
 constexpr int INFO = 16;                    // tiles that pages and masks are looked up ahead, in
 constexpr int BATCH = 8;                    // rounds of
-// What an item costs beside its tiles (loading Q, filling the pipeline, storing O), in tiles, by what the CTAs of one launch measured: with 2 for an 8-bit cache those with
-// nothing but short items took half as long again as the others.  Drafts (32 x 8 over 8192, e4m3): 170 us with 2, 140 with 4, 133 with 6; 64 sequences over
-// 16384 (BF16): 79.7 with 2, 77.8 with 3, 80.2 with 4.
+// What an item costs beside its tiles (loading Q, filling the pipeline, storing O), in tiles.  Times in us with 2 / 3 / 4 / 5 / 6:
+//                                                         BF16                        int8 (e4m3 within 1 us of it)
+//   drafts, 32 x 8 over 8192, heads of 128    109 / 99 / 92 / 88 / 90                 142 / 128 / 118 / 121 / 118
+//   the same, 4 heads of 256                   78 / 70 / 69 / 69 / 68                  91 / 86 / 86 / 86 / 87
+//   the same, heads of 64                      85 / 78 / 75 / 77 / 79                 118 / 108 / 100 / 106 / 105
+//   64 x 1 over 16384, heads of 128            80 / 79 / 82 / 84 / 88                 119 / 115 / 111 / 112 / 122
+//   64 x 1 over 8192, 2 heads of 256           46 / 44 / 44 / 44 / 45                  54 / 53 / 53 / 53 / 54
+//   13 x 1 over 30001, one head of 256         27 / 27 / 25 / 25 / 25                  32 / 32 / 30 / 30 / 30
+// 3 and 5 are within 12% of the best of every row.
 __host__ __device__ constexpr int overhead(int format) { return format == PI05_CACHE_BF16 ? 3 : 5; }
 constexpr int MAX_BATCH = 1024;
 constexpr float RESCALE = 8.0f;             // of exponents to the base 2: probabilities up to 256, their sums far from the ends of FP32
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(threads(FORMAT), 1) attention_kernel(const __g
         const uint32_t s_at = lanes + TM_S + sbuf * TILE, p_at = lanes + TM_P + buf * P_STEP;
         // A tile is read twice, CHUNK scores at a time: for the row's maximum, then for the probabilities.  (What the warps of a CTA execute per tile has to fit the
         // instruction cache.  With all 64 scores in registers 26% of the fetches missed it and drafts, 32 x 8 over 8192 in e4m3, took 245 us; read
-        // twice in 32s 14%, 142; in 16s and with the converters' loop rolled 121)
+        // twice in 32s 14%, 142; in 16s and with the converters' loop rolled 121, now 122 with a reference that goes by the keys that a row sees)
         auto load_chunk = [](uint32_t from, float (&x)[CHUNK]) {
           if constexpr (CHUNK == 32) ptx::tmem_ld_32x32(from, reinterpret_cast<uint32_t(&)[32]>(x));
           else ptx::tmem_ld_32x16(from, reinterpret_cast<uint32_t(&)[16]>(x));

@@ -98,7 +98,8 @@ class Pi05Prefill:
         ``positions`` int32 ``[batch, tokens]``.  Per layer their keys and values go into ``attention.cache``, at the end of the sequences that
         ``table`` int32 ``[batch, pages]`` and ``lengths`` int32 ``[batch]`` (with these tokens) describe, and the queries attend to the prefix and to
         their sequence; prefix, ``valid`` and ``causal`` as in ``SharedPrefixAttention.run``.  Returns the residual stream behind the last
-        layer, ``[batch, tokens, 2048]``; asynchronous on the current stream."""
+        layer, ``[batch, tokens, 2048]``, before the final norm; asynchronous on the current stream.  What tables and lengths hold that is out of range is
+        reported by ``attention.status()``."""
         if self.weights is None:
             raise _lib.EngineError(_lib.ERR_NOT_BOUND, self.lib.pi05_error_string(_lib.ERR_NOT_BOUND).decode())
         c = attention.cache
